@@ -1,7 +1,8 @@
 """The operators of an 8-bit KV cache and of speculative decoding, as they are measured.
 
 append  bf16 K and V rows quantised as they are written into an e4m3 cache: one power-of-two scale a row (token and
-        KV head), the smallest 2^e with max |x| <= 448 * 2^e
+        KV head), the smallest 2^e with max |x| <= 448 * 2^e; codes are [B, KV heads, rows, D], scale bytes [B, KV heads,
+        rows, 2] for K and V
 read    rows of an e4m3 cache read back as bf16
 attend  causal grouped-query attention over an e4m3 cache, sequences of different lengths in one call
 tree    attention of a tree of drafted tokens: each node over the context, its ancestors and itself; bf16 or e4m3 cache
@@ -150,7 +151,7 @@ def _inputs(case, seed):
     if kind == "keep":
         L, n = case["layers"], case["kept"]
         if case["e4m3"]:
-            codes = torch.randint(0, 0x7f, (2, L, B, cap, Hkv, D), generator=gen, device="cuda", dtype=torch.uint8)
+            codes = torch.randint(0, 0x7f, (2, L, B, Hkv, cap, D), generator=gen, device="cuda", dtype=torch.uint8)
             s.kc, s.vc = codes.view(torch.float8_e4m3fn)
             s.scales = torch.randint(100, 140, (L, B, Hkv, cap, 2), generator=gen, device="cuda", dtype=torch.uint8)
         else:
@@ -164,20 +165,19 @@ def _inputs(case, seed):
         return s
     if kind == "append":
         s.k, s.v = normal(B, S, Hkv, D), normal(B, S, Hkv, D)
-        s.kc = torch.zeros((B, cap, Hkv, D), device="cuda", dtype=torch.float8_e4m3fn)
+        s.kc = torch.zeros((B, Hkv, cap, D), device="cuda", dtype=torch.float8_e4m3fn)
         s.vc = torch.zeros_like(s.kc)
         s.scales = torch.full((B, Hkv, cap, 2), 127, device="cuda", dtype=torch.uint8)
         return s
     if kind != "read":
         s.q = normal(B, S, case["Hq"], D) * 2
         s.parents = _parents(case, gen) if kind == "tree" else None
-    kc, vc = normal(B, cap, Hkv, D), normal(B, cap, Hkv, D)
     if kind == "read" or case["e4m3"]:
-        s.kc, ks = _quantise(kc)
-        s.vc, vs = _quantise(vc)
-        s.scales = torch.stack([ks, vs], -1).transpose(1, 2).contiguous()
+        s.kc, ks = _quantise(normal(B, Hkv, cap, D))
+        s.vc, vs = _quantise(normal(B, Hkv, cap, D))
+        s.scales = torch.stack([ks, vs], -1)
     else:
-        s.kc, s.vc, s.scales = kc, vc, None
+        s.kc, s.vc, s.scales = normal(B, cap, Hkv, D), normal(B, cap, Hkv, D), None
     return s
 
 
@@ -202,8 +202,8 @@ def prepare(case, seed):
 # ---- the plain forms ------------------------------------------------------------------
 
 def _dequantise(codes, scale_bytes):
-    """float32 values [B, rows, Hkv, D] of codes and the scale bytes [B, Hkv, rows]."""
-    return torch.ldexp(codes.float(), scale_bytes.transpose(1, 2).unsqueeze(-1).int() - 127)
+    """float32 values [B, Hkv, rows, D] of codes and their scale bytes [B, Hkv, rows]."""
+    return torch.ldexp(codes.float(), scale_bytes.unsqueeze(-1).int() - 127)
 
 
 def _plain_append(s, c):
@@ -213,16 +213,16 @@ def _plain_append(s, c):
     start = s.lengths.long() if c["ragged"] else torch.zeros(B, device="cuda", dtype=torch.long)
     rows = start[:, None] + torch.arange(S, device="cuda")
     b = torch.arange(B, device="cuda")[:, None]
-    s.kc.view(torch.uint8)[b, rows] = kc.view(torch.uint8)
-    s.vc.view(torch.uint8)[b, rows] = vc.view(torch.uint8)
+    s.kc.view(torch.uint8).transpose(1, 2)[b, rows] = kc.view(torch.uint8)
+    s.vc.view(torch.uint8).transpose(1, 2)[b, rows] = vc.view(torch.uint8)
     s.scales.transpose(1, 2)[b, rows] = torch.stack([ks, vs], -1)
     return {"k": s.kc, "v": s.vc, "scales": s.scales.view(torch.float8_e8m0fnu)}
 
 
 def _plain_read(s, c):
     n = c["S"]
-    k = _dequantise(s.kc[:, :n], s.scales[:, :, :n, 0]).to(torch.bfloat16)
-    v = _dequantise(s.vc[:, :n], s.scales[:, :, :n, 1]).to(torch.bfloat16)
+    k = _dequantise(s.kc[:, :, :n], s.scales[:, :, :n, 0]).to(torch.bfloat16).transpose(1, 2)
+    v = _dequantise(s.vc[:, :, :n], s.scales[:, :, :n, 1]).to(torch.bfloat16).transpose(1, 2)
     if c["ragged"]:  # the rows behind a sequence stay as they are
         behind = (torch.arange(n, device="cuda") >= s.lengths[:, None])[:, :, None, None]
         k, v = torch.where(behind, s.k, k), torch.where(behind, s.v, v)
@@ -256,12 +256,13 @@ def _visible(s, c):
 def _plain_attend(s, c):
     B, S, cached, Hq, Hkv = c["B"], c["S"], c["cached"], c["Hq"], c["Hkv"]
     G = Hq // Hkv
-    k, v = s.kc[:, :cached], s.vc[:, :cached]
     if c["e4m3"]:
-        k = _dequantise(k, s.scales[:, :, :cached, 0])
-        v = _dequantise(v, s.scales[:, :, :cached, 1])
-    k = k.float().permute(0, 2, 3, 1).contiguous()                       # [B, Hkv, D, cached]
-    v = v.float().permute(0, 2, 1, 3).contiguous()
+        k = _dequantise(s.kc[:, :, :cached], s.scales[:, :, :cached, 0])
+        v = _dequantise(s.vc[:, :, :cached], s.scales[:, :, :cached, 1])
+    else:
+        k = s.kc[:, :cached].float().transpose(1, 2)
+        v = s.vc[:, :cached].float().transpose(1, 2).contiguous()
+    k = k.transpose(2, 3).contiguous()                                   # [B, Hkv, D, cached]
     q = s.q.float().view(B, S, Hkv, G, D).permute(0, 2, 1, 3, 4).reshape(B, Hkv, S * G, D)
     scores = torch.matmul(q, k).view(B, Hkv, S, G, cached) / math.sqrt(D)
     seen = _visible(s, c)[:, None, :, None, :]
@@ -283,11 +284,11 @@ def _plain_keep(s, c):
     b = torch.arange(B, device="cuda")[:, None]
     bits = torch.uint8 if c["e4m3"] else torch.bfloat16
     kc, vc = s.kc.view(bits), s.vc.view(bits)
+    if c["e4m3"]:
+        kc, vc, scales = kc.transpose(2, 3), vc.transpose(2, 3), s.scales.transpose(2, 3)  # [layers, B, rows, Hkv, ..]
+        scales[:, b, dst] = scales[:, b, src]
     kc[:, b, dst] = kc[:, b, src]
     vc[:, b, dst] = vc[:, b, src]
-    if c["e4m3"]:
-        rows = s.scales.transpose(2, 3)                                  # [layers, B, cap, Hkv, 2]
-        rows[:, b, dst] = rows[:, b, src]
     return _kept(s, c)
 
 
@@ -312,8 +313,9 @@ def _own(s, c):
                          stream=st)
         return {"k": s.k, "v": s.v}
     if kind == "keep":
-        q3k.kv_keep_path(p["kc"], p["vc"], p.get("scales"), c["layers"], B, cap, Hkv * D * (1 if c["e4m3"] else 2), Hkv, B,
-                         0, p["path"], c["kept"], starts=p["starts"], counts=p["counts"], stream=st)
+        heads, row = (Hkv, D) if c["e4m3"] else (1, 2 * Hkv * D)
+        q3k.kv_keep_path(p["kc"], p["vc"], p.get("scales"), c["layers"], B, heads, cap, row, B, 0, p["path"], c["kept"],
+                         starts=p["starts"], counts=p["counts"], stream=st)
         return _kept(s, c)
     cached, Hq = c["cached"], c["Hq"]
     if kind == "attend":
@@ -381,10 +383,10 @@ def _scale64(x):
 
 
 def _values64(s, b, h, n, which):
-    x = (s.kc, s.vc)[which][b, :n, h].double()
-    if s.scales is not None:
-        x = x * torch.exp2(s.scales[b, h, :n, which].double() - 127.0).unsqueeze(-1)
-    return x
+    x = (s.kc, s.vc)[which][b]
+    if s.scales is None:
+        return x[:n, h].double()
+    return x[h, :n].double() * torch.exp2(s.scales[b, h, :n, which].double() - 127.0).unsqueeze(-1)
 
 
 def _chain(parents):
@@ -409,7 +411,7 @@ def exact(case, seed):
         for i, (name, x) in enumerate((("k", s.k.double()), ("v", s.v.double()))):
             scale = _scale64(x)
             for b in range(B):
-                out[name][b, n[b]:n[b] + S] = x[b] / scale[b].unsqueeze(-1)
+                out[name][b, :, n[b]:n[b] + S] = (x[b] / scale[b].unsqueeze(-1)).transpose(0, 1)
                 out["scales"][b, :, n[b]:n[b] + S, i] = scale[b].t()
         return out
     if kind == "read":
@@ -425,10 +427,9 @@ def exact(case, seed):
         for b in range(B):
             for i in range(counts[b]):
                 to, at = start[b] + i, start[b] + path[b][i]
-                for x in (s.kc, s.vc):
-                    x[:, b, to] = x[:, b, at].clone()
-                if case["e4m3"]:
-                    s.scales[:, b, :, to] = s.scales[:, b, :, at].clone()
+                for x in (s.kc, s.vc, s.scales) if case["e4m3"] else (s.kc, s.vc):
+                    rows = x[:, b].transpose(1, 2) if case["e4m3"] else x[:, b]
+                    rows[:, to] = rows[:, at].clone()
         out = {"k": s.kc.double(), "v": s.vc.double()}
         if case["e4m3"]:
             out["scales"] = torch.exp2(s.scales.double() - 127.0)
