@@ -21,6 +21,7 @@
  *   rope         x1' = RNE(x1*c - x2*s), x2' = RNE(x2*c + x1*s), pairs (p, p + D/2)
  *   add_rms_norm h = RNE(h + d); y = rms_norm(h) computed from the rounded h
  *   qk_norm_rope per head: n = rms_norm(x) (two roundings), then rope(n)
+ *   e4m3 cache   code = RNE(x / scale), scale a power of two (below)
  */
 #ifndef Q3K_ABI_H
 #define Q3K_ABI_H
@@ -327,6 +328,144 @@ Q3K_API int q3k_qk_norm_rope_kv_append_bf16(uint16_t *q, const uint16_t *k,
                           const int32_t *positions, uint16_t *k_cache,
                           uint16_t *v_cache, int64_t seq_cap,
                           int64_t cache_start, q3k_stream_t stream);
+
+/*
+ * The e4m3 KV cache: one layer's K and V in 8 bits.
+ *   k_codes, v_codes  [batch_cap, Hkv, seq_cap, D], one OCP e4m3 byte a value
+ *   scales            [batch_cap, Hkv, seq_cap, 2], the bytes of the K row and
+ *                     the V row of that position; byte s stands for 2^(s - 127)
+ * A row (one position, one KV head) holds x[d] = code[d] * scale.  It is
+ * written with the smallest scale 2^e, e >= -126, for which no finite |x[d]|
+ * exceeds 448 * 2^e, and code = RNE(x * 2^-e); the scaling is exact, so the
+ * code's rounding (half a step, 2^-4 of the value) is the only one, and every
+ * value read back is a bf16 value.  An infinity or a NaN becomes a NaN code
+ * (e4m3 has no infinity) and does not count for the scale.  Scale bytes 0 and
+ * 255 are never written.  A head's rows lie together (in the bf16 cache a
+ * position's heads do): attention reads one head's rows, 5.4-5.9 TB/s so and
+ * 4.9-5.7 with the heads of a position together.  The reference has no such
+ * cache.
+ */
+
+/*
+ * Quantising KV-cache append: K and V [B, S, Hkv, D] bf16 (contiguous) go to
+ * rows start .. start + S - 1 of batch rows 0 .. B - 1 of an e4m3 cache layer,
+ * or with starts (device int32 [B]) to rows starts[b] .. starts[b] + S - 1;
+ * start is then not used, and rows outside [0, seq_cap) are not written.
+ * start + S > seq_cap is Q3K_ERR_OUT_OF_RANGE.  Beside q3k_kv_append, which
+ * copies the bytes.
+ */
+Q3K_API int q3k_kv_append_e4m3_bf16(const uint16_t *key, const uint16_t *value,
+                          uint8_t *k_codes, uint8_t *v_codes,
+                          uint8_t *scales, int64_t B, int64_t S, int32_t Hkv,
+                          int32_t D, int64_t seq_cap, int64_t start,
+                          const int32_t *starts, q3k_stream_t stream);
+
+/*
+ * Rows first .. first + count - 1 of batch rows 0 .. B - 1 of an e4m3 cache
+ * layer as bf16, key / value [B, count, Hkv, D] (exact: code * scale is a bf16
+ * value; below 2^-126 it is rounded to bf16's subnormals).  With lengths
+ * (device int32 [B]) the output rows of positions at or past lengths[b] are
+ * left as they were.  first + count > seq_cap is Q3K_ERR_OUT_OF_RANGE.
+ */
+Q3K_API int q3k_kv_read_e4m3_bf16(const uint8_t *k_codes, const uint8_t *v_codes,
+                          const uint8_t *scales, uint16_t *key,
+                          uint16_t *value, int64_t B, int32_t Hkv, int32_t D,
+                          int64_t seq_cap, int64_t first, int64_t count,
+                          const int32_t *lengths, q3k_stream_t stream);
+
+/*
+ * Causal grouped-query attention over an e4m3 cache layer, sequences of
+ * different lengths in one call.  q, out [B, S, Hq * D] bf16.  Sequence b has
+ * n = lengths[b] cached rows (device int32 [B]; NULL: every one has `cached`),
+ * of which the last S are those of its queries: query (b, s) attends to rows
+ * 0 .. n - S + s; query head h reads KV head h / (Hq / Hkv); scale
+ * 1 / sqrt(D).  A query without a row (n - S + s < 0) gets zeros; a sequence
+ * whose length lies outside [0, cached] gets NaN (the kernel reads nothing
+ * there).  `cached` is what the host knows of the longest sequence, at most
+ * seq_cap, and with lengths == NULL at least S: the launch is laid out for it,
+ * so one captured in a graph serves every step up to it.  head_dim 128 with
+ * 16-byte aligned q and codes and 2-byte aligned scales takes the matrix-core
+ * kernels, anything up to 256 the generic one.  workspace (16-byte aligned
+ * device memory, may be NULL) of at least
+ * q3k_cache_attention_workspace_bytes(...) bytes lets a launch split the key
+ * range and merge the slices.  Calls that share a workspace must not overlap.
+ */
+Q3K_API int q3k_gqa_attention_e4m3_bf16(const uint16_t *q, const uint8_t *k_codes,
+                          const uint8_t *v_codes, const uint8_t *scales,
+                          uint16_t *out, int64_t B, int64_t S, int32_t Hq,
+                          int32_t Hkv, int32_t D, int64_t seq_cap,
+                          int64_t cached, const int32_t *lengths,
+                          void *workspace, int64_t workspace_bytes,
+                          q3k_stream_t stream);
+
+/*
+ * Attention of trees of drafted tokens over a bf16 KV cache.  q, out
+ * [B, T, Hq * D] bf16, T <= 256 nodes a sequence, whose K and V are already in
+ * the cache: of the n = lengths[b] rows of sequence b (device int32 [B]; NULL:
+ * `cached` of each) the last T are its nodes', in their order, and the n - T
+ * before them the context.  parents (device int32, sequence b's T at
+ * parents + b * parents_stride; parents_stride 0: one tree for all): the
+ * parent of node t, in [0, t), or -1 for a node right after the context.  Node
+ * t attends to the context, its ancestors and itself.  -2 marks a node that is
+ * not there (trees of different sizes in a batch): it and its descendants get
+ * zeros.  A node whose way up meets any other number gets NaN, as does a
+ * sequence whose length is neither 0 (zeros) nor in [T, cached].  What rows
+ * hold that a node does not attend to, NaN included, does not reach it.
+ * k_cache / v_cache are views as those of q3k_gqa_attention_bf16, [B, cached,
+ * Hkv, D] by element strides; `cached` and the workspace are as in
+ * q3k_gqa_attention_e4m3_bf16; the fast kernels take head_dim 128 with unit dim
+ * stride and 16-byte aligned rows.
+ */
+Q3K_API int q3k_gqa_tree_attention_bf16(const uint16_t *q, const uint16_t *k_cache,
+                          const uint16_t *v_cache, uint16_t *out,
+                          const int32_t *parents, int64_t parents_stride,
+                          int64_t B, int64_t T, int32_t Hq, int32_t Hkv,
+                          int32_t D, int64_t cached, const int32_t *lengths,
+                          const int64_t *k_strides, const int64_t *v_strides,
+                          void *workspace, int64_t workspace_bytes,
+                          q3k_stream_t stream);
+
+/* The same over an e4m3 cache layer. */
+Q3K_API int q3k_gqa_tree_attention_e4m3_bf16(const uint16_t *q,
+                          const uint8_t *k_codes, const uint8_t *v_codes,
+                          const uint8_t *scales, uint16_t *out,
+                          const int32_t *parents, int64_t parents_stride,
+                          int64_t B, int64_t T, int32_t Hq, int32_t Hkv,
+                          int32_t D, int64_t seq_cap, int64_t cached,
+                          const int32_t *lengths, void *workspace,
+                          int64_t workspace_bytes, q3k_stream_t stream);
+
+/*
+ * Workspace bytes that let the three attention calls above split the key range
+ * of up to `cached` rows (S queries or tree nodes a sequence; 0: they split
+ * none): one of the size for the cache's length serves every shorter one of the
+ * same B, S and heads.
+ */
+Q3K_API int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S,
+                          int32_t Hq, int32_t Hkv, int32_t D, int64_t cached);
+
+/*
+ * Keeps the rows of accepted drafted tokens: in every layer of a KV cache, row
+ * start + path[b, i] of sequence b moves to row start + i, for i in
+ * [0, counts[b]) (device int32 [B], at most path_len; NULL: path_len of each).
+ * path (device int32 [B, path_len]) holds each sequence's accepted nodes; with
+ * starts (device int32 [B]) sequence b's rows begin at starts[b] and start is
+ * not used.  All rows are read before any is written, as far as the caller can
+ * tell.  A node is never moved up: an entry with path[b, i] < i, or one whose
+ * row lies past the cache, leaves row start + i as it was, and a start outside
+ * [0, seq_cap) the whole sequence.
+ * key_cache / value_cache: [layers, batch_cap, heads, seq_cap, row_bytes], the
+ * bytes copied unchanged: a bf16 or fp32 cache [layers, batch_cap, seq_cap,
+ * Hkv, D] has heads = 1 and row_bytes of a whole position, an e4m3 cache
+ * heads = Hkv and row_bytes = D, and its scales [layers, batch_cap, heads,
+ * seq_cap, 2] move along (NULL: none).  B <= batch_cap.
+ */
+Q3K_API int q3k_kv_keep_path(void *key_cache, void *value_cache, uint8_t *scales,
+                          int64_t layers, int64_t batch_cap, int32_t heads,
+                          int64_t seq_cap, int64_t row_bytes, int64_t B,
+                          int64_t start, const int32_t *path, int64_t path_len,
+                          const int32_t *starts, const int32_t *counts,
+                          q3k_stream_t stream);
 
 /*
  * Host-side RoPE table: cache[p, i, 0] = (float)cos(p * theta^(-2i/D)),

@@ -99,6 +99,15 @@ SIGNATURES = {
     "q3k_kv_append": [_p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p],
     "q3k_qk_norm_rope_kv_append_bf16": [_p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _f32, _p, _i64, _i64, _p,
                                         _p, _p, _i64, _i64, _p],
+    "q3k_kv_append_e4m3_bf16": [_p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i64, _i64, _p, _p],
+    "q3k_kv_read_e4m3_bf16": [_p, _p, _p, _p, _p, _i64, _i32, _i32, _i64, _i64, _i64, _p, _p],
+    "q3k_gqa_attention_e4m3_bf16": [_p, _p, _p, _p, _p, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _p, _p, _i64, _p],
+    "q3k_gqa_tree_attention_bf16": [_p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _p, _p, _p, _p, _i64,
+                                    _p],
+    "q3k_gqa_tree_attention_e4m3_bf16": [_p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _p, _p,
+                                         _i64, _p],
+    "q3k_cache_attention_workspace_bytes": [_i64, _i64, _i32, _i32, _i32, _i64],
+    "q3k_kv_keep_path": [_p, _p, _p, _i64, _i64, _i32, _i64, _i64, _i64, _i64, _p, _i64, _p, _p, _p],
     "q3k_build_rope_cache_f32": [_p, _i64, _i32, _f32],
 }
 
@@ -353,6 +362,77 @@ def qk_norm_rope_kv_append(q, k, v, qw, kw, B, S, Hq, Hkv, D, eps, cache, P, sta
         st = load().q3k_qk_norm_rope_kv_append_bf16(_ptr(q), _ptr(k), _ptr(v), _ptr(qw), _ptr(kw), B, S, Hq, Hkv, D,
                                                     eps, _ptr(cache), P, start, _ptr(positions), _ptr(k_cache),
                                                     _ptr(v_cache), seq_cap, cache_start, _ptr(stream))
+    _check(st)
+
+
+def kv_append_e4m3(k, v, k_codes, v_codes, scales, B, S, Hkv, D, seq_cap, start, starts=None, stream=None):
+    """Into an e4m3 cache layer: codes [batch_cap, Hkv, seq_cap, D], scale bytes [batch_cap, Hkv, seq_cap, 2]."""
+    st = _fast().q3k_kv_append_e4m3_bf16(k, v, k_codes, v_codes, scales, B, S, Hkv, D, seq_cap, start, starts, stream)
+    if st is None:
+        st = load().q3k_kv_append_e4m3_bf16(_ptr(k), _ptr(v), _ptr(k_codes), _ptr(v_codes), _ptr(scales), B, S, Hkv, D,
+                                            seq_cap, start, _ptr(starts), _ptr(stream))
+    _check(st)
+
+
+def kv_read_e4m3(k_codes, v_codes, scales, k, v, B, Hkv, D, seq_cap, first, count, lengths=None, stream=None):
+    st = _fast().q3k_kv_read_e4m3_bf16(k_codes, v_codes, scales, k, v, B, Hkv, D, seq_cap, first, count, lengths, stream)
+    if st is None:
+        st = load().q3k_kv_read_e4m3_bf16(_ptr(k_codes), _ptr(v_codes), _ptr(scales), _ptr(k), _ptr(v), B, Hkv, D,
+                                          seq_cap, first, count, _ptr(lengths), _ptr(stream))
+    _check(st)
+
+
+def gqa_attention_e4m3(q, k_codes, v_codes, scales, out, B, S, Hq, Hkv, D, seq_cap, cached, lengths=None, stream=None,
+                       workspace=None, workspace_bytes=0):
+    """lengths: the cached rows of each sequence (int32 [B] on the device), at most ``cached``; None: ``cached`` of each."""
+    st = _fast().q3k_gqa_attention_e4m3_bf16(q, k_codes, v_codes, scales, out, B, S, Hq, Hkv, D, seq_cap, cached, lengths,
+                                             workspace, workspace_bytes, stream)
+    if st is None:
+        st = load().q3k_gqa_attention_e4m3_bf16(_ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(scales), _ptr(out), B, S, Hq,
+                                                Hkv, D, seq_cap, cached, _ptr(lengths), _ptr(workspace), workspace_bytes,
+                                                _ptr(stream))
+    _check(st)
+
+
+def gqa_tree_attention(q, k_cache, v_cache, out, parents, parents_stride, B, T, Hq, Hkv, D, cached, k_strides, v_strides,
+                       lengths=None, stream=None, workspace=None, workspace_bytes=0):
+    """k_strides / v_strides: 4 element strides (batch, position, head, dim) of the cache views."""
+    st = _fast().q3k_gqa_tree_attention_bf16(q, k_cache, v_cache, out, parents, parents_stride, B, T, Hq, Hkv, D, cached,
+                                             lengths, k_strides, v_strides, workspace, workspace_bytes, stream)
+    if st is None:
+        ks = (ctypes.c_int64 * 4)(*[int(x) for x in k_strides])
+        vs = (ctypes.c_int64 * 4)(*[int(x) for x in v_strides])
+        st = load().q3k_gqa_tree_attention_bf16(_ptr(q), _ptr(k_cache), _ptr(v_cache), _ptr(out), _ptr(parents),
+                                                parents_stride, B, T, Hq, Hkv, D, cached, _ptr(lengths),
+                                                ctypes.cast(ks, _p), ctypes.cast(vs, _p), _ptr(workspace),
+                                                workspace_bytes, _ptr(stream))
+    _check(st)
+
+
+def gqa_tree_attention_e4m3(q, k_codes, v_codes, scales, out, parents, parents_stride, B, T, Hq, Hkv, D, seq_cap, cached,
+                            lengths=None, stream=None, workspace=None, workspace_bytes=0):
+    st = _fast().q3k_gqa_tree_attention_e4m3_bf16(q, k_codes, v_codes, scales, out, parents, parents_stride, B, T, Hq, Hkv,
+                                                  D, seq_cap, cached, lengths, workspace, workspace_bytes, stream)
+    if st is None:
+        st = load().q3k_gqa_tree_attention_e4m3_bf16(_ptr(q), _ptr(k_codes), _ptr(v_codes), _ptr(scales), _ptr(out),
+                                                     _ptr(parents), parents_stride, B, T, Hq, Hkv, D, seq_cap, cached,
+                                                     _ptr(lengths), _ptr(workspace), workspace_bytes, _ptr(stream))
+    _check(st)
+
+
+def cache_attention_workspace_bytes(B, S, Hq, Hkv, D, cached):
+    """For gqa_attention_e4m3, gqa_tree_attention and gqa_tree_attention_e4m3 (S: queries or nodes a sequence)."""
+    return int(load().q3k_cache_attention_workspace_bytes(B, S, Hq, Hkv, D, cached))
+
+
+def kv_keep_path(k_cache, v_cache, scales, layers, batch_cap, heads, seq_cap, row_bytes, B, start, path, path_len,
+                 starts=None, counts=None, stream=None):
+    """Caches [layers, batch_cap, heads, seq_cap, row_bytes]; scales of an e4m3 cache, else None."""
+    st = _fast().q3k_kv_keep_path(k_cache, v_cache, scales, layers, batch_cap, heads, seq_cap, row_bytes, B, start, path,
+                                  path_len, starts, counts, stream)
+    if st is None:
+        st = load().q3k_kv_keep_path(_ptr(k_cache), _ptr(v_cache), _ptr(scales), layers, batch_cap, heads, seq_cap,
+                                     row_bytes, B, start, _ptr(path), path_len, _ptr(starts), _ptr(counts), _ptr(stream))
     _check(st)
 
 

@@ -88,6 +88,9 @@ namespace q3k
     // 32768 keys the estimate below wanted more for two.
     constexpr int64_t kAttDecodeMaxBlocks = 2048;
 
+    // Most nodes of a sequence's tree of drafted tokens.
+    constexpr int32_t kTreeMaxNodes = 256;
+
     struct AttnSplit
     {
         int32_t splits = 1;

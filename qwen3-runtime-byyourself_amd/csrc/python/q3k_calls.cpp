@@ -39,7 +39,7 @@ namespace
         return false;
     }
 
-    // Four element strides, as the attention entry point takes them.
+    // Four element strides, as the attention entry points take them.
     struct Strides
     {
         int64_t v[4];
@@ -149,6 +149,13 @@ namespace
                           q3k_stream_t>(args, n);
     }
 
+    PyObject *tree_attention(PyObject *, PyObject *const *args, Py_ssize_t n)
+    {
+        return call_typed<&q3k_gqa_tree_attention_bf16, const uint16_t *, const uint16_t *, const uint16_t *, uint16_t *,
+                          const int32_t *, int64_t, int64_t, int64_t, int32_t, int32_t, int32_t, int64_t, const int32_t *,
+                          Strides, Strides, void *, int64_t, q3k_stream_t>(args, n);
+    }
+
 #define Q3K_ENTRY(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<&name>)), METH_FASTCALL, nullptr}
     PyMethodDef g_methods[] = {
         Q3K_ENTRY(q3k_embedding_bf16),
@@ -169,6 +176,13 @@ namespace
         Q3K_ENTRY(q3k_topk_candidates_bf16),
         Q3K_ENTRY(q3k_kv_append),
         Q3K_ENTRY(q3k_qk_norm_rope_kv_append_bf16),
+        Q3K_ENTRY(q3k_kv_append_e4m3_bf16),
+        Q3K_ENTRY(q3k_kv_read_e4m3_bf16),
+        Q3K_ENTRY(q3k_gqa_attention_e4m3_bf16),
+        {"q3k_gqa_tree_attention_bf16", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&tree_attention)),
+         METH_FASTCALL, nullptr},
+        Q3K_ENTRY(q3k_gqa_tree_attention_e4m3_bf16),
+        Q3K_ENTRY(q3k_kv_keep_path),
         {nullptr, nullptr, 0, nullptr},
     };
 
