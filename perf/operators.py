@@ -192,6 +192,8 @@ def prepare(case, seed):
         s.stream = torch.cuda.current_stream().cuda_stream
         if case["kind"] in ("attend", "tree"):
             s.out = torch.empty_like(s.q)
+            if s.parents is not None:
+                s.parents = s.parents.to(torch.int32)  # as the call takes them
             s.ws_bytes = s.q3k.cache_attention_workspace_bytes(case["B"], case["S"], case["Hq"], case["Hkv"], D,
                                                                case["cached"])
             s.ws = torch.empty(s.ws_bytes, device="cuda", dtype=torch.uint8) if s.ws_bytes else None
