@@ -8,9 +8,30 @@
 // n - T + t and those of its ancestors (tree).  A query that sees no row gets
 // zeros, a sequence whose length is out of range NaN.
 //
+// Matrix-core paths (head_dim 128, 16-byte rows), built from the tile operations of
+// attention_tiles.hpp, whose mathematics they share with the causal bf16 attention:
+// S^T = K Q^T, online softmax, O^T += V^T P^T, keys in tiles, up to 32 (position,
+// head) columns to a wave.
+//   Few columns (at most 32 to a (sequence, KV head): decode, small trees): the
+//   block's waves divide the keys and stream their own tiles through LDS.  A tile
+//   of the e4m3 cache is 64 keys of 128 bytes; its codes stay 8 bits wide until a
+//   fragment is in registers: K's with ds_read_b128, 16 dims of a key, converted
+//   to two bf16 fragments with the key's scale (a lane holds one key, so the scale
+//   is one register); V's with the 8-bit transpose read, 8 keys of a dim, converted
+//   without a scale, which is multiplied into the weights instead (there a lane
+//   holds one column and 16 keys of each 32).
+//   More columns (larger trees, prefill): a block of waves shares its K and V tiles
+//   as bf16; codes are converted once, on their way into LDS.
+// The mask only touches the tiles at a sequence's end.  A masked score is -inf, so
+// what K holds in a row that a query does not see never counts.  What V holds there
+// meets a weight of zero, and zero times an infinity or a NaN is NaN: so a masked
+// tile is looked through for such values, and if there is one its product goes the
+// careful way (pv_careful).
+//
 // Generic path (any head_dim <= 256, any strides and alignment): one wave per
 // query row, its rows in order, lanes over the head dimension, the running
 // maximum and sum of the softmax in fp32.
+#include "attention_tiles.hpp"
 #include "dispatch.hpp"
 #include "kv_e4m3.hpp"
 
@@ -38,6 +59,14 @@ namespace q3k
             int32_t D;
             float scale;
             int64_t rows;
+            // the fast kernels: query blocks of a pair, slices of split_keys rows, their
+            // results (unnormalised O^T [splits, rows, D], reference max and sum
+            // [splits, rows, 2])
+            int32_t qblocks;
+            int32_t splits;
+            int32_t split_keys;
+            float *part_o;
+            float *part_ml;
         };
 
         constexpr int kTreeWords = kTreeMaxNodes / 64;
@@ -176,6 +205,1037 @@ namespace q3k
             }
         }
 
+        // ---- masks -----------------------------------------------------------------
+
+        // The masks of a block's positions in a tree: word w + 1 of a position holds
+        // the bits of nodes 32 w .. + 31 that it sees, word 0 stands for the context
+        // before them and the last word for what lies behind.
+        template <bool TREE, int POSITIONS, int NODES>
+        struct TreeMasks
+        {
+            static constexpr int kWords = NODES / 32 + 2;
+            int32_t parent[NODES];
+            uint32_t mask[POSITIONS][kWords];
+            int32_t state[POSITIONS];
+        };
+        template <int POSITIONS, int NODES>
+        struct TreeMasks<false, POSITIONS, NODES>
+        {
+        };
+
+        // Positions first .. first + count - 1 of a tree of T nodes; every thread of the
+        // block calls it.
+        template <int POSITIONS, int NODES>
+        __device__ __forceinline__ void tree_masks(TreeMasks<true, POSITIONS, NODES> &t, const int32_t *parents, int T, int first,
+                                                   int count, int thread, int threads)
+        {
+            for (int i = thread; i < T; i += threads)
+                t.parent[i] = parents[i];
+            constexpr int W = TreeMasks<true, POSITIONS, NODES>::kWords;
+            for (int i = thread; i < count * W; i += threads)
+                t.mask[i / W][i % W] = i % W == 0 ? 0xffffffffu : 0u;
+            __syncthreads();
+            for (int i = thread; i < count; i += threads)
+            {
+                uint32_t *row = t.mask[i];
+                t.state[i] = static_cast<int32_t>(
+                    walk_up(t.parent, first + i, [&](int32_t u) { row[1 + u / 32] |= 1u << (u % 32); }));
+            }
+            __syncthreads();
+        }
+
+        // Which of the 32 keys from `off` nodes into the tree (below 0: the context) a
+        // position sees.
+        template <int W>
+        __device__ __forceinline__ uint32_t tree_window(const uint32_t (&row)[W], int32_t off)
+        {
+            int i = (off >> 5) + 1, j = i + 1;
+            i = i < 0 ? 0 : i < W ? i : W - 1;
+            j = j < 0 ? 0 : j < W ? j : W - 1;
+            return __builtin_amdgcn_alignbit(row[j], row[i], static_cast<uint32_t>(off) & 31u);
+        }
+
+        // Which of the 32 keys from key0 are at most `last`.
+        __device__ __forceinline__ uint32_t causal_window(int32_t key0, int32_t last)
+        {
+            const int32_t n = last - key0 + 1;
+            return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
+        }
+
+        // The bit of element r of a lane's S^T half in its window.
+        __device__ __forceinline__ uint32_t element_bit(int r, int lg) { return 1u << (8 * (r / 4) + 4 * lg + r % 4); }
+
+        template <int HH>
+        __device__ __forceinline__ void mask_scores(f32x16_t (&sacc)[HH], const uint32_t (&seen)[HH], int lg)
+        {
+#pragma unroll
+            for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((seen[hh] & element_bit(r, lg)) == 0)
+                        sacc[hh][r] = -__builtin_huge_valf();
+        }
+
+        // ---- products over e4m3 tiles ------------------------------------------------
+
+        typedef int i32x2_t __attribute__((ext_vector_type(2)));
+        typedef __attribute__((address_space(3))) i32x2_t lds_i32x2_t;
+
+        // Slots of the 16-byte chunks of a 128-byte row of codes.  Two rows span the LDS
+        // banks, so K's chunks move by the row's pair: 16 consecutive rows put a chunk in
+        // 16 places.  V's transpose reads take rows {0..3, 8..11} or {4..7, 12..15} of 16
+        // and two chunks at once: bits 1 and 3 of the row spread the four pairs of rows.
+        __device__ __forceinline__ int k_slot8(int r, int c) { return c ^ ((r >> 1) & 7); }
+        __device__ __forceinline__ int v_slot8(int r, int c) { return c ^ ((r & 2) | ((r >> 1) & 4)); }
+
+        // S^T of the 64 keys of a tile of codes; scale[hh]: that of key 32 hh + li.  A
+        // lane's 16 codes of chunk 2 c + lg are the dims of Q fragments 2 c and 2 c + 1
+        // (load_q orders them so).
+        template <typename Next>
+        __device__ __forceinline__ void qk_codes(const unsigned char *k_lds, const bf16x8_t (&qf)[kAttD / 16], int li, int lg,
+                                                 const float (&scale)[2], f32x16_t (&sacc)[2], Next next)
+        {
+            auto read = [&](int c, int hh) __attribute__((always_inline)) {
+                return *reinterpret_cast<const uint4 *>(k_lds + (32 * hh + li) * kAttD + 16 * k_slot8(li, 2 * c + lg));
+            };
+            sacc[0] = f32x16_t{};
+            sacc[1] = f32x16_t{};
+            uint4 codes[2][2] = {{read(0, 0), read(0, 1)}, {}};
+#pragma unroll
+            for (int c = 0; c < kAttD / 32; ++c)
+            {
+                if (c + 1 < kAttD / 32)
+                {
+                    codes[(c + 1) % 2][0] = read(c + 1, 0);
+                    codes[(c + 1) % 2][1] = read(c + 1, 1);
+                }
+                else
+                    next();
+                __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+                {
+                    const uint4 w = codes[c % 2][hh];
+                    sacc[hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.x, w.y), scale[hh])), qf[2 * c],
+                                                                       sacc[hh], 0, 0, 0);
+                    sacc[hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.z, w.w), scale[hh])),
+                                                                       qf[2 * c + 1], sacc[hh], 0, 0, 0);
+                }
+            }
+        }
+
+        // Per-lane LDS offsets of V's 8-bit transpose reads: lanes 2 i, 2 i + 1 of each 16
+        // give row i of the eight keys 4 lg + 0..3, 8 + 4 lg + 0..3 (those of the P^T
+        // elements a lane holds) and 16 dims; a lane gets the eight keys of its dim.
+        __device__ __forceinline__ void v_offsets8(int lane, int (&v_off)[kAttD / 32])
+        {
+            const int j = lane % 16, lg = lane / 32, i = j / 2;
+            const int row = 8 * (i / 4) + 4 * lg + i % 4;
+#pragma unroll
+            for (int dt = 0; dt < kAttD / 32; ++dt)
+                v_off[dt] = row * kAttD + 16 * v_slot8(row, 2 * dt + (lane / 16) % 2) + 8 * (j % 2);
+        }
+
+        // Fragment of P V step i (16-key chunk i / 4, dims 32 (i % 4) .. + 31), in codes.
+        __device__ __forceinline__ uint2 read_v8(const unsigned char *v_lds, const int (&v_off)[kAttD / 32], int i)
+        {
+            const i32x2_t c = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i32x2_t *)(v_lds + v_off[i % 4] + 16 * (i / 4) * kAttD));
+            return make_uint2(static_cast<uint32_t>(c.x), static_cast<uint32_t>(c.y));
+        }
+
+        __device__ __forceinline__ void pv_codes(const unsigned char *v_lds, const int (&v_off)[kAttD / 32],
+                                                 const bf16x8_t (&phi)[2][2], const bf16x8_t (&plo)[2][2], f32x16_t (&o)[kAttD / 32])
+        {
+            uint2 vq[kAhead + 1];
+#pragma unroll
+            for (int x = 0; x < kAhead; ++x)
+                vq[x] = read_v8(v_lds, v_off, x);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+            {
+                if (i + kAhead < 16)
+                    vq[(i + kAhead) % (kAhead + 1)] = read_v8(v_lds, v_off, i + kAhead);
+                __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
+                const int dt = i % 4, hh = i / 8, mm = (i / 4) % 2;
+                const bf16x8_t v = as_bf8(decode8(vq[i % (kAhead + 1)], 1.0f));
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, phi[hh][mm], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, plo[hh][mm], o[dt], 0, 0, 0);
+            }
+        }
+
+        // ---- masked tiles that hold infinities or NaN ---------------------------------
+
+        // Whether a wave's lanes see such a value among the `bytes` of a V tile.
+        template <bool CODES>
+        __device__ __forceinline__ bool has_nonfinite(const unsigned char *v_lds, int bytes, int lane)
+        {
+            constexpr uint32_t kAbs = CODES ? 0x7f7f7f7fu : 0x7f807f80u, kOne = CODES ? 0x01010101u : 0x00800080u;
+            constexpr uint32_t kTop = CODES ? 0x80808080u : 0x80008000u;
+            uint32_t top = 0;
+            for (int i = 16 * lane; i < bytes; i += 16 * kWave)
+            {
+                const uint4 w = *reinterpret_cast<const uint4 *>(v_lds + i);
+                top |= ((w.x & kAbs) + kOne) | ((w.y & kAbs) + kOne) | ((w.z & kAbs) + kOne) | ((w.w & kAbs) + kOne);
+            }
+            return __any((top & kTop) != 0);
+        }
+
+        // O^T += V^T P^T of a masked tile with infinities or NaN in it: the product with
+        // those set to zero, then, key by key, each of them added where its column sees
+        // the key.  Rare, so it is written for few registers: read(i) is the bf16 fragment
+        // of P V step i, values(key, dt, q4) the four V values of a key at dims
+        // 32 dt + 8 q4 + 4 lg, those of elements 4 q4 .. + 3 of O^T.
+        template <int HH, typename Read, typename Values>
+        __device__ __forceinline__ void pv_careful(Read read, Values values, const uint32_t (&seen)[HH], const bf16x8_t (&phi)[HH][2],
+                                                   const bf16x8_t (&plo)[HH][2], f32x16_t (&o)[kAttD / 32])
+        {
+#pragma unroll
+            for (int i = 0; i < 8 * HH; ++i)
+            {
+                const int dt = i % 4, hh = i / 8, mm = (i / 4) % 2;
+                Vec8 v = __builtin_bit_cast(Vec8, read(i));
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                {
+                    const uint32_t bad = ((v.d[j] & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+                    v.d[j] &= ~((bad >> 15) * 0xffffu);
+                }
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v), phi[hh][mm], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(v), plo[hh][mm], o[dt], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+#pragma unroll 1
+            for (int key = 0; key < 32 * HH; ++key)
+            {
+                const bool sees = ((key < 32 ? seen[0] : seen[HH - 1]) >> (key % 32) & 1u) != 0;
+#pragma unroll
+                for (int dt = 0; dt < kAttD / 32; ++dt)
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                    {
+                        const float4 x = values(key, dt, q4);
+                        const float e[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            o[dt][4 * q4 + u] +=
+                                sees && (__float_as_uint(e[u]) & 0x7f800000u) == 0x7f800000u ? e[u] : 0.0f;
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+            }
+        }
+
+        // The values argument of pv_careful: of a tile of bf16 rows, and of codes.
+        __device__ __forceinline__ float4 v_values(const unsigned char *v_lds, int lg, int key, int dt, int q4)
+        {
+            const uint2 w = *reinterpret_cast<const uint2 *>(v_lds + key * kRowBytes + 16 * v_slot(key, 4 * dt + q4) + 8 * lg);
+            return make_float4(bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y));
+        }
+        __device__ __forceinline__ float4 v_values8(const unsigned char *v_lds, int lg, int key, int dt, int q4)
+        {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(v_lds + key * kAttD + 16 * v_slot8(key, 2 * dt + q4 / 2) +
+                                                                   8 * (q4 % 2) + 4 * lg);
+            const uint32_t lo = decode2<false>(w, 1.0f), hi = decode2<true>(w, 1.0f);
+            return make_float4(bf_lo(lo), bf_hi(lo), bf_lo(hi), bf_hi(hi));
+        }
+
+        // ---- results -------------------------------------------------------------------
+
+        // Q fragments of the lane's column, a padding column's from the last position
+        // (its results are not stored).  CODES: in the order of qk_codes.
+        template <bool CODES>
+        __device__ __forceinline__ void load_q(const CacheArgs &a, int64_t b, int32_t s_col, int h_col, int lg,
+                                               bf16x8_t (&qf)[kAttD / 16])
+        {
+            const int64_t s_row = s_col < a.S ? s_col : a.S - 1;
+            const Vec8 *qrow = reinterpret_cast<const Vec8 *>(a.q + ((b * a.S + s_row) * a.Hq + h_col) * kAttD);
+#pragma unroll
+            for (int c = 0; c < kAttD / 16; ++c)
+                qf[c] = as_bf8(qrow[CODES ? 4 * (c / 2) + 2 * lg + c % 2 : 2 * c + lg]);
+        }
+
+        // Dims 32 dt .. + 31 of a query's result: bf16 O / l, or with slices the
+        // unnormalised O^T of this one.
+        __device__ __forceinline__ void store_dims(const CacheArgs &a, bool split, int sp, int64_t row, int dt, int lg,
+                                                   const f32x16_t &o, float inv, float l, Query q)
+        {
+            if (split)
+            {
+                float *po = a.part_o + (static_cast<int64_t>(sp) * a.rows + row) * kAttD;
+#pragma unroll
+                for (int q4 = 0; q4 < 4; ++q4)
+                {
+                    float4 w = {o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]};
+                    if (q != Query::Sees)
+                        w = {0.0f, 0.0f, 0.0f, 0.0f};
+                    *reinterpret_cast<float4 *>(po + dt * 32 + 8 * q4 + 4 * lg) = w;
+                }
+                return;
+            }
+            const bool none = q != Query::Sees || l == 0.0f;
+            const uint32_t fill = q == Query::Bad ? 0x7fc07fc0u : 0u;
+            uint16_t *orow = a.out + row * kAttD;
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+            {
+                uint2 w;
+                w.x = pack_rne(o[4 * q4] * inv, o[4 * q4 + 1] * inv);
+                w.y = pack_rne(o[4 * q4 + 2] * inv, o[4 * q4 + 3] * inv);
+                if (none)
+                    w.x = w.y = fill;
+                *reinterpret_cast<uint2 *>(orow + dt * 32 + 8 * q4 + 4 * lg) = w;
+            }
+        }
+        // The slice's reference max and sum: those of a query without a row leave it
+        // zeros, those of a bad one NaN.
+        __device__ __forceinline__ void store_ml(const CacheArgs &a, int sp, int64_t row, float m, float l, Query q)
+        {
+            const float2 ml = q == Query::Sees    ? make_float2(m, l)
+                              : q == Query::Empty ? make_float2(-__builtin_huge_valf(), 0.0f)
+                                                  : make_float2(0.0f, __builtin_nanf(""));
+            reinterpret_cast<float2 *>(a.part_ml)[static_cast<int64_t>(sp) * a.rows + row] = ml;
+        }
+
+        // Zeros or NaN for columns col0 .. col_end - 1 of a pair (a sequence without
+        // rows, or a block whose queries see none).
+        __device__ __forceinline__ void fill_columns(const CacheArgs &a, int64_t b, int kvh, int32_t col0, int32_t col_end, bool nan,
+                                                     int thread, int threads)
+        {
+            const int g = a.Hq / a.Hkv;
+            const uint32_t w = nan ? 0x7fc07fc0u : 0u;
+            for (int32_t i = thread; i < (col_end - col0) * (kAttD / 4); i += threads)
+            {
+                const int32_t col = col0 + i / (kAttD / 4);
+                const int64_t row = (b * a.S + col / g) * a.Hq + kvh * g + col % g;
+                reinterpret_cast<uint2 *>(a.out + row * kAttD)[i % (kAttD / 4)] = make_uint2(w, w);
+            }
+        }
+
+        // ---- few columns ---------------------------------------------------------------
+
+        // At most 32 columns to a (sequence, KV head): one wave holds them all, the
+        // block's KW waves divide the keys and share nothing until the merge.  Each
+        // streams its own tiles (8 KiB of K and of V: 64 keys of codes or 32 of bf16)
+        // through two K and two V buffers with no barrier, as the causal bf16 attention
+        // does; the scales of a tile's rows come along, a word a key.
+        template <int KW, bool E4M3, bool TREE>
+        __global__ __launch_bounds__(KW *kWave) void cache_decode_kernel(CacheArgs a)
+        {
+            constexpr int RB = E4M3 ? kAttD : kRowBytes, HH = E4M3 ? 2 : 1, kKeys = 32 * HH, kTileBytes = kKeys * RB;
+            using St = Staging<1, kKeys, RB>;
+            constexpr int kL = St::kLoads, kS = E4M3 ? 1 : 0;
+            __shared__ __attribute__((aligned(16))) unsigned char k_a[KW * kTileBytes];
+            __shared__ __attribute__((aligned(16))) unsigned char k_b[KW * kTileBytes];
+            __shared__ __attribute__((aligned(16))) unsigned char v_a[KW * kTileBytes];
+            __shared__ __attribute__((aligned(16))) unsigned char v_b[KW * kTileBytes];
+            __shared__ uint32_t s_a[E4M3 ? KW * kWave : 1];
+            __shared__ uint32_t s_b[E4M3 ? KW * kWave : 1];
+            __shared__ __attribute__((aligned(16))) float v_scale[E4M3 ? KW * kWave : 4];
+            __shared__ TreeMasks<TREE, kAttColsPerWave, kAttColsPerWave> tree;
+            const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+            const int lane = threadIdx.x % kWave;
+            const int li = lane % 32, lg = lane / 32;
+            // slices of a pair side by side
+            const int sp = static_cast<int>(blockIdx.x) % a.splits, pair = static_cast<int>(blockIdx.x) / a.splits;
+            const int kvh = pair % a.Hkv;
+            const int64_t b = pair / a.Hkv;
+            const int32_t S = static_cast<int32_t>(a.S);
+            const int g = a.Hq / a.Hkv;
+            bool bad;
+            const int32_t n_keys = sequence_rows(a, b, bad);
+            if (n_keys == 0)
+            {
+                if (sp == 0)
+                    fill_columns(a, b, kvh, 0, S * g, bad, threadIdx.x, KW * kWave);
+                return;
+            }
+            const int64_t slice_begin = static_cast<int64_t>(sp) * a.split_keys;
+            if (slice_begin >= n_keys)
+                return;
+            const int32_t k_begin = static_cast<int32_t>(slice_begin);
+            const bool split = n_keys > a.split_keys;
+            const int32_t k_end = n_keys - k_begin > a.split_keys ? k_begin + a.split_keys : n_keys;
+            const int first = k_begin / kKeys + kw, tile_end = (k_end + kKeys - 1) / kKeys;
+            const int mine = first < tile_end ? (tile_end - first + KW - 1) / KW : 0;
+            const int32_t context = n_keys - S;                       // rows before the queries' own
+            const int32_t all_seen = TREE ? context : context + 1;    // rows every query sees
+
+            if constexpr (TREE)
+                tree_masks(tree, a.parents + b * a.parents_stride, S, 0, S, threadIdx.x, KW * kWave);
+            // the lane's column; lanes past the last one repeat a row of the last position
+            const int32_t s_col = li / g;
+            const int h_col = kvh * g + li % g;
+            const bool col_ok = s_col < S;
+            const int32_t s_row = col_ok ? s_col : S - 1;
+            Query query = Query::Sees;
+            if constexpr (TREE)
+                query = static_cast<Query>(tree.state[s_row]);
+
+            constexpr int64_t kElement = E4M3 ? 1 : 2;
+            const unsigned char *kbase = static_cast<const unsigned char *>(a.k) + (b * a.ks0 + kvh * a.ks2) * kElement;
+            const unsigned char *vbase = static_cast<const unsigned char *>(a.v) + (b * a.vs0 + kvh * a.vs2) * kElement;
+            const uint8_t *sbase = a.scales + 2 * (b * a.ss0 + kvh * a.ss2);
+            const int32_t kstride = static_cast<int32_t>(a.ks1 * kElement), vstride = static_cast<int32_t>(a.vs1 * kElement);
+            const auto kslot = [](int r, int c) __attribute__((always_inline)) { return E4M3 ? k_slot8(r, c) : k_slot(r, c); };
+            const auto vslot = [](int r, int c) __attribute__((always_inline)) { return E4M3 ? v_slot8(r, c) : v_slot(r, c); };
+            int32_t k_voff[kL], v_voff[kL];
+            tile_offsets<1, kKeys, RB>(0, lane, kstride, kslot, k_voff);
+            tile_offsets<1, kKeys, RB>(0, lane, vstride, vslot, v_voff);
+            auto load_k = [&](int j, unsigned char *buf, uint32_t *sbuf) __attribute__((always_inline)) {
+                const int tile = first + KW * j;
+                if constexpr (E4M3)
+                {
+                    const int last = n_keys - 1 - tile * kKeys;
+                    __builtin_amdgcn_raw_ptr_buffer_load_lds(tile_rsrc(sbase + 2 * static_cast<int64_t>(tile) * kKeys),
+                                                             (lds_void_t *)(sbuf + kw * kWave), 2, 2 * (lane < last ? lane : last), 0,
+                                                             0, 0);
+                }
+                load_tile_rows<1, kKeys, RB>(tile, buf + kw * kTileBytes, kbase, kstride, n_keys, 0, lane, k_voff, kslot);
+            };
+            auto load_v = [&](int j, unsigned char *buf) __attribute__((always_inline)) {
+                load_tile_rows<1, kKeys, RB>(first + KW * j, buf + kw * kTileBytes, vbase, vstride, n_keys, 0, lane, v_voff, vslot);
+            };
+            bf16x8_t qf[kAttD / 16];
+            load_q<E4M3>(a, b, s_col, h_col, lg, qf);
+            __asm__ volatile("" ::: "memory"); // Q first: waiting for it waits for no tile
+            if (mine > 0)
+            {
+                load_k(0, k_a, s_a);
+                load_v(0, v_a);
+            }
+            if (mine > 1)
+            {
+                load_k(1, k_b, s_b);
+                load_v(1, v_b);
+            }
+            int v_off[kAttD / 32];
+            if constexpr (E4M3)
+                v_offsets8(lane, v_off);
+            else
+                v_offsets(lane, v_off);
+            f32x16_t o[kAttD / 32];
+#pragma unroll
+            for (int dt = 0; dt < kAttD / 32; ++dt)
+                o[dt] = f32x16_t{};
+            float m = -__builtin_huge_valf(), l = 0.0f;
+            const float scale2 = a.scale * kLog2e;
+
+            auto step = [&](int j, unsigned char *kb, unsigned char *vb, uint32_t *sb) __attribute__((always_inline)) {
+                const unsigned char *k_lds = kb + kw * kTileBytes, *v_lds = vb + kw * kTileBytes;
+                float *vs = v_scale + (E4M3 ? kw * kWave : 0);
+                // loads by age: K(j) with its scales, V(j), K(j + 1), V(j + 1)
+                if (j + 1 < mine)
+                    wait_loads<3 * kL + kS>();
+                else
+                    wait_loads<kL>();
+                f32x16_t sacc[HH];
+                if constexpr (E4M3)
+                {
+                    // lane i has the scales of key i: K's go to the lanes that hold the key's
+                    // codes, i and i + 32 (one swap gives both halves), V's to LDS.  A row
+                    // past the end may hold any byte; 254 keeps its scale finite.
+                    const uint32_t pair_bytes = sb[kw * kWave + lane];
+                    const uint32_t vbyte = pair_bytes >> 8;
+                    vs[lane] = e4m3_scale(vbyte < 254u ? vbyte : 254u);
+                    const uint32_t ks = (pair_bytes & 255u) << 23;
+                    const auto halves = __builtin_amdgcn_permlane32_swap(ks, ks, false, false);
+                    const float k_scale[2] = {__uint_as_float(halves[0]), __uint_as_float(halves[1])};
+                    qk_codes(k_lds, qf, li, lg, k_scale, sacc, []() __attribute__((always_inline)) {});
+                }
+                else
+                    qk_tile<HH>(k_lds, qf, li, lg, sacc, [](int) __attribute__((always_inline)) {});
+                wait_loads<63>();
+                if (j + 2 < mine)
+                    load_k(j + 2, kb, sb);
+                const int32_t key0 = (first + KW * j) * kKeys;
+                const bool masked = key0 + kKeys > all_seen;
+                uint32_t seen[HH];
+                if (masked)
+                {
+#pragma unroll
+                    for (int hh = 0; hh < HH; ++hh)
+                    {
+                        if constexpr (TREE)
+                            seen[hh] = tree_window(tree.mask[s_row], key0 + 32 * hh - context);
+                        else
+                            seen[hh] = causal_window(key0 + 32 * hh, context + s_row);
+                    }
+                    mask_scores<HH>(sacc, seen, lg);
+                }
+                bf16x8_t phi[HH][2], plo[HH][2];
+                float alpha;
+                if constexpr (E4M3)
+                {
+                    float4 w[HH][4];
+#pragma unroll
+                    for (int hh = 0; hh < HH; ++hh)
+#pragma unroll
+                        for (int q4 = 0; q4 < 4; ++q4)
+                            w[hh][q4] = *reinterpret_cast<const float4 *>(vs + 32 * hh + 8 * q4 + 4 * lg);
+                    alpha = softmax_tile<HH>(sacc, scale2, m, l, phi, plo, [&](float p, int hh, int r) __attribute__((always_inline)) {
+                        const float4 &x = w[hh][r / 4];
+                        return p * (r % 4 == 0 ? x.x : r % 4 == 1 ? x.y : r % 4 == 2 ? x.z : x.w);
+                    });
+                }
+                else
+                    alpha = softmax_tile<HH>(sacc, scale2, m, l, phi, plo);
+                rescale(o, alpha);
+                // V(j), then K(j + 1), V(j + 1), K(j + 2)
+                if (j + 2 < mine)
+                    wait_loads<3 * kL + 2 * kS>();
+                else if (j + 1 < mine)
+                    wait_loads<2 * kL + kS>();
+                else
+                    wait_loads<0>();
+                // one query sees every row up to its own, and past it only repeats of that row
+                if (masked && S > 1 && has_nonfinite<E4M3>(v_lds, kTileBytes, lane))
+                {
+                    pv_careful<HH>(
+                        [&](int i) __attribute__((always_inline)) {
+                            if constexpr (E4M3)
+                                return as_bf8(decode8(read_v8(v_lds, v_off, i), 1.0f));
+                            else
+                                return read_v(v_lds, v_off, i);
+                        },
+                        [&](int key, int dt, int q4) __attribute__((always_inline)) {
+                            return E4M3 ? v_values8(v_lds, lg, key, dt, q4) : v_values(v_lds, lg, key, dt, q4);
+                        },
+                        seen, phi, plo, o);
+                }
+                else if constexpr (E4M3)
+                    pv_codes(v_lds, v_off, phi, plo, o);
+                else
+                {
+                    bf16x8_t vq[kAhead + 1];
+#pragma unroll
+                    for (int x = 0; x < kAhead; ++x)
+                        vq[x] = read_v(v_lds, v_off, x);
+                    pv_tile<HH>(v_lds, v_off, phi, plo, o, vq);
+                }
+                wait_loads<63>();
+                if (j + 2 < mine)
+                    load_v(j + 2, vb);
+            };
+            for (int j = 0; j < mine; j += 2)
+            {
+                step(j, k_a, v_a, s_a);
+                if (j + 1 < mine)
+                    step(j + 1, k_b, v_b, s_b);
+            }
+            const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
+            const auto put_dims = [&](int dt, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+                if (col_ok)
+                    store_dims(a, split, sp, row, dt, lg, part, inv, sum, query);
+            };
+            const auto put_ml = [&](float mx, float sum) __attribute__((always_inline)) {
+                if (split && col_ok)
+                    store_ml(a, sp, row, mx, sum, query);
+            };
+            if constexpr (KW == 1)
+            {
+#pragma unroll
+                for (int dt = 0; dt < kAttD / 32; ++dt)
+                    put_dims(dt, o[dt], 1.0f / l, l);
+                if (lg == 0)
+                    put_ml(m, l);
+            }
+            else
+            {
+                __syncthreads(); // every wave is done with its tiles
+                merge_groups<1, KW>(k_a, k_b, v_a, v_b, 0, kw, li, lg, o, m, l, put_dims, put_ml);
+            }
+        }
+
+        // ---- more columns ---------------------------------------------------------------
+
+        // As the block kernel of the causal bf16 attention: CW waves side by side over the
+        // columns, KW groups of them dividing the keys, the P V product of a tile beside
+        // the S^T product of the next; with a mask of its own and a length for each
+        // sequence.
+        //   bf16: two K and two V buffers, filled straight from memory, one barrier a
+        //   tile.
+        //   e4m3: one K and one V buffer of bf16, filled from staged codes.  Each wave
+        //   stages 16 rows of K and of V (2 KiB each, the same lanes that convert them, so
+        //   no barrier stands between), a tile ahead.  When every wave is past a step's
+        //   products both buffers are free, and K of the next tile and V of this one are
+        //   converted into them: two barriers a tile, half the LDS for tiles and no
+        //   registers for loads in flight (holding the codes in registers instead spilled
+        //   or cost the second block of a CU).
+        template <int CW, int KW, int HH, bool E4M3, bool TREE>
+        __global__ __launch_bounds__(CW *KW *kWave, 2) void cache_block_kernel(CacheArgs a)
+        {
+            const int g = a.Hq / a.Hkv;
+            constexpr int kBlockCols = 32 * CW;
+            constexpr int kKeys = 32 * HH;
+            constexpr int kTileBytes = kKeys * kRowBytes;
+            constexpr int kWaves = CW * KW;
+            constexpr int kRows = kKeys / CW, kCodeLoads = kRows / 8, kCodeBytes = kRows * kAttD; // of a wave
+            static_assert(kRows == 16, "rows of a wave");
+            // the groups' merge takes 4 KiB a wave of each buffer
+            constexpr int kSecond = !E4M3 ? KW * kTileBytes : KW > 1 ? kWaves * 4096 : kWaves * kCodeBytes;
+            __shared__ __attribute__((aligned(16))) unsigned char k_a[KW * kTileBytes];
+            __shared__ __attribute__((aligned(16))) unsigned char k_b[kSecond]; // e4m3: the staged codes
+            __shared__ __attribute__((aligned(16))) unsigned char v_a[KW * kTileBytes];
+            __shared__ __attribute__((aligned(16))) unsigned char v_b[kSecond];
+            __shared__ uint32_t k_scales[E4M3 ? kWaves * kWave : 1];
+            __shared__ uint32_t v_scales[E4M3 ? kWaves * kWave : 1];
+            __shared__ TreeMasks<TREE, kBlockCols, kTreeMaxNodes> tree;
+
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+            const int cw = wave % CW, kw = wave / CW;
+            const int lane = threadIdx.x % kWave;
+            const int li = lane % 32, lg = lane / 32;
+            // the pair runs fastest (one XCD holds a pair's K and V), the query blocks of a
+            // slice longest first, slices outermost
+            const int pairs = static_cast<int>(gridDim.x) / (a.qblocks * a.splits);
+            const int pair = static_cast<int>(blockIdx.x) % pairs;
+            const int rest = static_cast<int>(blockIdx.x) / pairs;
+            const int sp = rest / a.qblocks, qb = a.qblocks - 1 - rest % a.qblocks;
+            const int kvh = pair % a.Hkv;
+            const int64_t b = pair / a.Hkv;
+            const int32_t S = static_cast<int32_t>(a.S);
+            const int32_t n_cols = S * g;
+            const int32_t block_col = qb * kBlockCols;
+            const int32_t block_end = n_cols - block_col > kBlockCols ? block_col + kBlockCols : n_cols;
+            const int32_t s_first = block_col / g, s_last = (block_end - 1) / g;
+            bool bad;
+            const int32_t n = sequence_rows(a, b, bad);
+            const int32_t context = n - S;
+            // rows the block's queries see between them
+            const int32_t n_keys = n == 0 || TREE ? n : context + s_last + 1;
+            if (n_keys <= 0)
+            {
+                if (sp == 0)
+                    fill_columns(a, b, kvh, block_col, block_end, bad, threadIdx.x, kWaves * kWave);
+                return;
+            }
+            const int64_t slice_begin = static_cast<int64_t>(sp) * a.split_keys;
+            if (slice_begin >= n_keys)
+                return;
+            const int32_t k_begin = static_cast<int32_t>(slice_begin);
+            const bool split = n_keys > a.split_keys;
+            const int32_t k_end = n_keys - k_begin < a.split_keys ? n_keys : k_begin + a.split_keys;
+            // tiles of the block [tile0, tile_end); this group's: first, first + KW, ...
+            const int tile_end = (k_end + kKeys - 1) / kKeys;
+            const int tile0 = k_begin / kKeys;
+            const int first = tile0 + kw;
+            const int steps = (tile_end - tile0 + KW - 1) / KW;
+            const int mine = first < tile_end ? (tile_end - first + KW - 1) / KW : 0;
+
+            if constexpr (TREE)
+                tree_masks(tree, a.parents + b * a.parents_stride, S, s_first, s_last - s_first + 1, threadIdx.x, kWaves * kWave);
+            // this lane's column
+            const int32_t wave_col = block_col + 32 * cw;
+            const int32_t col = wave_col + li;
+            const bool col_ok = col < n_cols;
+            const int32_t s_col = col / g;
+            const int h_col = kvh * g + col % g;
+            const int32_t s_row = col_ok ? s_col : S - 1;
+            const bool wave_active = wave_col < n_cols;
+            // rows that every query of the wave sees
+            const int32_t all_seen = TREE ? context : context + wave_col / g + 1;
+
+            constexpr int64_t kElement = E4M3 ? 1 : 2;
+            const unsigned char *kbase = static_cast<const unsigned char *>(a.k) + (b * a.ks0 + kvh * a.ks2) * kElement;
+            const unsigned char *vbase = static_cast<const unsigned char *>(a.v) + (b * a.vs0 + kvh * a.vs2) * kElement;
+            const uint8_t *sbase = a.scales + 2 * (b * a.ss0 + kvh * a.ss2);
+            const int32_t kstride = static_cast<int32_t>(a.ks1 * kElement), vstride = static_cast<int32_t>(a.vs1 * kElement);
+            const auto kslot = [](int r, int c) __attribute__((always_inline)) { return k_slot(r, c); };
+            const auto vslot = [](int r, int c) __attribute__((always_inline)) { return v_slot(r, c); };
+            // bf16: rows straight into a tile
+            int32_t k_voff[Staging<CW, kKeys>::kLoads], v_voff[Staging<CW, kKeys>::kLoads];
+            if constexpr (!E4M3)
+            {
+                tile_offsets<CW, kKeys>(cw, lane, kstride, kslot, k_voff);
+                tile_offsets<CW, kKeys>(cw, lane, vstride, vslot, v_voff);
+            }
+            auto load_k = [&](int tile, unsigned char *buf) __attribute__((always_inline)) {
+                load_tile_rows<CW, kKeys>(tile, buf + kw * kTileBytes, kbase, kstride, n_keys, cw, lane, k_voff, kslot);
+            };
+            auto load_v = [&](int tile, unsigned char *buf) __attribute__((always_inline)) {
+                load_tile_rows<CW, kKeys>(tile, buf + kw * kTileBytes, vbase, vstride, n_keys, cw, lane, v_voff, vslot);
+            };
+            // e4m3: the wave's rows kRows cw .. + 15 of a tile, eight lanes a row of codes; a
+            // lane's 16 codes land at 16 * lane and go to chunks 2 (lane % 8) and the next
+            auto stage = [&](int tile, const unsigned char *base, unsigned char *codes, uint32_t *scales) __attribute__((always_inline)) {
+                const int32_t row0 = tile * kKeys + kRows * cw, end = n_keys - 1;
+                // based at the tile's first row, which the sequence has; rows past its end
+                // repeat the last
+                const int32_t key0 = tile * kKeys;
+                auto past = [&](int32_t r) __attribute__((always_inline)) { return (row0 + r < end ? row0 + r : end) - key0; };
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(tile_rsrc(sbase + 2 * static_cast<int64_t>(key0)),
+                                                         (lds_void_t *)(scales + wave * kWave), 2, 2 * past(lane % 16), 0, 0, 0);
+                const __amdgpu_buffer_rsrc_t rs = tile_rsrc(base + static_cast<int64_t>(key0) * kAttD);
+#pragma unroll
+                for (int x = 0; x < kCodeLoads; ++x)
+                    dma16(rs, past(8 * x + lane / 8) * kAttD + 16 * (lane % 8), codes + wave * kCodeBytes + x * 1024);
+            };
+            auto convert = [&](const unsigned char *codes, const uint32_t *scales, int shift, unsigned char *buf, auto slot)
+                __attribute__((always_inline)) {
+#pragma unroll
+                for (int x = 0; x < kCodeLoads; ++x)
+                {
+                    const uint4 c = *reinterpret_cast<const uint4 *>(codes + wave * kCodeBytes + x * 1024 + 16 * lane);
+                    const uint32_t byte = (scales[wave * kWave + 8 * x + lane / 8] >> shift) & 255u;
+                    // a row past the end may hold any byte; 254 keeps its scale finite
+                    const float scale = e4m3_scale(byte < 254u ? byte : 254u);
+                    const int r = kRows * cw + 8 * x + lane / 8;
+                    unsigned char *row = buf + kw * kTileBytes + r * kRowBytes;
+                    *reinterpret_cast<Vec8 *>(row + 16 * slot(r, 2 * (lane % 8))) = decode8(make_uint2(c.x, c.y), scale);
+                    *reinterpret_cast<Vec8 *>(row + 16 * slot(r, 2 * (lane % 8) + 1)) = decode8(make_uint2(c.z, c.w), scale);
+                }
+            };
+            bf16x8_t qf[kAttD / 16];
+            load_q<false>(a, b, s_col, h_col, lg, qf);
+            int v_off[kAttD / 32];
+            v_offsets(lane, v_off);
+            f32x16_t o[kAttD / 32];
+#pragma unroll
+            for (int dt = 0; dt < kAttD / 32; ++dt)
+                o[dt] = f32x16_t{};
+            float m = -__builtin_huge_valf(), l = 0.0f;
+            const float scale2 = a.scale * kLog2e;
+            bf16x8_t phi[HH][2], plo[HH][2]; // P of the tile whose P V is still to be issued
+            bool masked = false;             // whether that is a masked tile
+
+            // which of a tile's keys the lane's column sees
+            auto seen_keys = [&](int32_t key0, uint32_t (&seen)[HH]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int hh = 0; hh < HH; ++hh)
+                {
+                    if constexpr (TREE)
+                        seen[hh] = tree_window(tree.mask[s_row - s_first], key0 + 32 * hh - context);
+                    else
+                        seen[hh] = causal_window(key0 + 32 * hh, context + s_row);
+                }
+            };
+            // the careful P V of the previous tile, if it needs it
+            auto careful = [&](const unsigned char *v_lds, int32_t key0) __attribute__((always_inline)) {
+                if (!masked || !has_nonfinite<false>(v_lds, kTileBytes, lane))
+                    return false;
+                uint32_t seen[HH];
+                seen_keys(key0, seen);
+                pv_careful<HH>([&](int i) __attribute__((always_inline)) { return read_v(v_lds, v_off, i); },
+                               [&](int key, int dt, int q4) __attribute__((always_inline)) {
+                                   return v_values(v_lds, lg, key, dt, q4);
+                               },
+                               seen, phi, plo, o);
+                return true;
+            };
+            auto pv = [&](const unsigned char *v_lds, bf16x8_t (&vq)[kAhead + 1]) __attribute__((always_inline)) {
+                pv_tile<HH>(v_lds, v_off, phi, plo, o, vq);
+            };
+            // The products of a step: S^T of this tile, P V of the previous one (WITH_PV).
+            auto products = [&](auto with_pv, int32_t key0, const unsigned char *k_lds, const unsigned char *v_lds,
+                                f32x16_t (&sacc)[HH]) __attribute__((always_inline)) {
+                constexpr bool kPv = decltype(with_pv)::value;
+                bool done = !kPv;
+                if constexpr (kPv)
+                    done = careful(v_lds, key0 - KW * kKeys);
+                __builtin_amdgcn_s_setprio(1);
+                bf16x8_t vq[kAhead + 1];
+                qk_tile<HH>(k_lds, qf, li, lg, sacc, [&](int x) __attribute__((always_inline)) {
+                    if constexpr (kPv)
+                        vq[x] = read_v(v_lds, v_off, x);
+                });
+                masked = key0 + kKeys > all_seen;
+                if (masked)
+                {
+                    uint32_t seen[HH];
+                    seen_keys(key0, seen);
+                    mask_scores<HH>(sacc, seen, lg);
+                }
+                if constexpr (kPv)
+                    if (!done)
+                        pv(v_lds, vq);
+                __builtin_amdgcn_s_setprio(0);
+            };
+            auto softmax = [&](const f32x16_t (&sacc)[HH]) __attribute__((always_inline)) {
+                const float alpha = softmax_tile<HH>(sacc, scale2, m, l, phi, plo);
+                // o holds the tiles before this one at the previous reference
+                rescale(o, alpha);
+            };
+            using no_pv = std::integral_constant<bool, false>;
+            using with_pv = std::integral_constant<bool, true>;
+            if constexpr (E4M3)
+            {
+                auto step = [&](auto pv_too, int j) __attribute__((always_inline)) {
+                    const bool active = wave_active && (KW == 1 || j < mine);
+                    f32x16_t sacc[HH];
+                    if (active)
+                        products(pv_too, (first + KW * j) * kKeys, k_a + kw * kTileBytes, v_a + kw * kTileBytes, sacc);
+                    wait_loads<0>();
+                    __syncthreads(); // every wave is past the products: both tiles are free
+                    if (j + 1 < mine)
+                        convert(k_b, k_scales, 0, k_a, kslot);
+                    if (j < mine)
+                        convert(v_b, v_scales, 8, v_a, vslot);
+                    wait_loads<63>(); // the staged codes are read
+                    if (j + 2 < mine)
+                        stage(first + KW * (j + 2), kbase, k_b, k_scales);
+                    if (j + 1 < mine)
+                        stage(first + KW * (j + 1), vbase, v_b, v_scales);
+                    if (active)
+                        softmax(sacc);
+                    __syncthreads();
+                };
+                if (mine > 0)
+                {
+                    stage(first, kbase, k_b, k_scales);
+                    stage(first, vbase, v_b, v_scales);
+                }
+                wait_loads<0>();
+                if (mine > 0)
+                    convert(k_b, k_scales, 0, k_a, kslot);
+                wait_loads<63>();
+                if (mine > 1)
+                    stage(first + KW, kbase, k_b, k_scales);
+                __syncthreads();
+                step(no_pv{}, 0);
+                for (int j = 1; j < steps; ++j)
+                    step(with_pv{}, j);
+            }
+            else
+            {
+                // K of the next tile loads while this one is computed, V of it after the
+                // barrier, into the buffer the step has finished with
+                auto step = [&](auto pv_too, int j, unsigned char *k_cur, unsigned char *k_next, unsigned char *v_prev)
+                    __attribute__((always_inline)) {
+                    const int tile = first + KW * j;
+                    if (j + 1 < mine)
+                        load_k(tile + KW, k_next);
+                    if (wave_active && (KW == 1 || j < mine))
+                    {
+                        f32x16_t sacc[HH];
+                        products(pv_too, tile * kKeys, k_cur + kw * kTileBytes, v_prev + kw * kTileBytes, sacc);
+                        softmax(sacc);
+                    }
+                    wait_loads<0>();
+                    __syncthreads();
+                    if (j + 1 < mine)
+                        load_v(tile + KW, v_prev);
+                };
+                if (mine > 0)
+                {
+                    load_k(first, k_a);
+                    load_v(first, v_a);
+                }
+                wait_loads<0>();
+                __syncthreads();
+                // V of step j sits in v_a when j is even, else in v_b
+                step(no_pv{}, 0, k_a, k_b, v_b);
+                for (int j = 1; j < steps; j += 2)
+                {
+                    step(with_pv{}, j, k_b, k_a, v_a);
+                    if (j + 1 < steps)
+                        step(with_pv{}, j + 1, k_a, k_b, v_b);
+                }
+            }
+            if (wave_active && mine > 0)
+            {
+                const unsigned char *v_lds = (E4M3 || (mine - 1) % 2 == 0 ? v_a : v_b) + kw * kTileBytes;
+                if (!careful(v_lds, (first + KW * (mine - 1)) * kKeys))
+                {
+                    bf16x8_t vq[kAhead + 1];
+#pragma unroll
+                    for (int x = 0; x < kAhead; ++x)
+                        vq[x] = read_v(v_lds, v_off, x);
+                    pv(v_lds, vq);
+                }
+            }
+
+            Query query = Query::Sees;
+            if constexpr (TREE)
+                query = static_cast<Query>(tree.state[s_row - s_first]);
+            const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
+            const auto put_dims = [&](int dt, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+                if (col_ok)
+                    store_dims(a, split, sp, row, dt, lg, part, inv, sum, query);
+            };
+            const auto put_ml = [&](float mx, float sum) __attribute__((always_inline)) {
+                if (split && col_ok)
+                    store_ml(a, sp, row, mx, sum, query);
+            };
+            if constexpr (KW == 1)
+            {
+#pragma unroll
+                for (int dt = 0; dt < kAttD / 32; ++dt)
+                    put_dims(dt, o[dt], 1.0f / l, l);
+                if (lg == 0)
+                    put_ml(m, l);
+            }
+            else
+            {
+                __syncthreads(); // every wave is done with the V tiles
+                merge_groups<CW, KW>(k_a, k_b, v_a, v_b, cw, kw, li, lg, o, m, l, put_dims, put_ml);
+            }
+        }
+
+        // ---- merging slices ---------------------------------------------------------------
+
+        // WPR waves to a query row: lane i of each reads slice i's reference max and sum,
+        // wave w the unnormalised O^T of slices w, w + WPR, ... (all loads of a round
+        // before any is used); weights 2^(m_i - max m), then sum w O / sum w l.  A row
+        // whose query block fits one slice is already done.
+        constexpr int kMergeWaves = 4;
+        constexpr int kMergeRound = kAttMaxSplits / kMergeWaves;
+
+        template <int WPR>
+        __global__ __launch_bounds__(kMergeWaves *kWave) void cache_merge_kernel(CacheArgs a, int32_t block_cols)
+        {
+            static_assert(WPR == 1 || WPR == kMergeWaves, "waves per row");
+            __shared__ float2 wave_acc[kMergeWaves][kWave];
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+            const int lane = threadIdx.x % kWave;
+            const int part = WPR == 1 ? 0 : wave;
+            const int64_t row = WPR == 1 ? static_cast<int64_t>(blockIdx.x) * kMergeWaves + wave : blockIdx.x;
+            if (row >= a.rows)
+                return; // whole waves, and with one row a wave no barrier below
+            const uint32_t r32 = static_cast<uint32_t>(row), hq = static_cast<uint32_t>(a.Hq), S = static_cast<uint32_t>(a.S);
+            const uint32_t bs = r32 / hq, h = r32 - bs * hq, b = bs / S;
+            const int32_t s = static_cast<int32_t>(bs - b * S);
+            bool bad;
+            const int32_t n = sequence_rows(a, b, bad);
+            if (n == 0)
+                return;
+            int32_t own = n; // rows this query's slices reach
+            if (a.parents == nullptr)
+            {
+                const int32_t g = a.Hq / a.Hkv, col = s * g + static_cast<int32_t>(h) % g;
+                const int64_t last = ((static_cast<int64_t>(col) / block_cols + 1) * block_cols - 1) / g;
+                const int32_t s_last = last < a.S ? static_cast<int32_t>(last) : static_cast<int32_t>(a.S) - 1;
+                own = n - static_cast<int32_t>(a.S) + s + 1;
+                if (own + s_last - s <= a.split_keys)
+                    return;
+            }
+            else if (n <= a.split_keys)
+                return;
+            const int splits = own <= 0 ? 1 : (own - 1) / a.split_keys + 1;
+            float2 ml = make_float2(-__builtin_huge_valf(), 0.0f);
+            if (lane < splits)
+                ml = reinterpret_cast<const float2 *>(a.part_ml)[static_cast<int64_t>(lane) * a.rows + row];
+            float a0 = 0.0f, a1 = 0.0f, w = 0.0f;
+            auto round = [&](int s0) __attribute__((always_inline)) {
+                float2 v[kMergeRound];
+#pragma unroll
+                for (int u = 0; u < kMergeRound; ++u)
+                {
+                    const int sp = s0 + part + WPR * u;
+                    if (sp < splits)
+                        v[u] = reinterpret_cast<const float2 *>(a.part_o + (static_cast<int64_t>(sp) * a.rows + row) * kAttD)[lane];
+                }
+                if (s0 == 0)
+                {
+                    float mx = ml.x;
+#pragma unroll
+                    for (int off = kWave / 2; off > 0; off /= 2)
+                        mx = fmaxf(mx, __shfl_xor(mx, off, kWave));
+                    mx = mx == -__builtin_huge_valf() ? 0.0f : mx;
+                    w = lane < splits ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
+                }
+#pragma unroll
+                for (int u = 0; u < kMergeRound; ++u)
+                {
+                    const int sp = s0 + part + WPR * u;
+                    if (sp < splits)
+                    {
+                        const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), sp));
+                        a0 += ws * v[u].x;
+                        a1 += ws * v[u].y;
+                    }
+                }
+            };
+            round(0);
+            if constexpr (WPR == 1)
+                for (int s0 = kMergeRound; s0 < splits; s0 += kMergeRound)
+                    round(s0);
+            const float lsum = group_sum<kWave>(w * ml.y);
+            if constexpr (WPR > 1)
+            {
+                wave_acc[wave][lane] = make_float2(a0, a1);
+                __syncthreads();
+                if (part != 0)
+                    return;
+#pragma unroll
+                for (int k = 1; k < WPR; ++k)
+                {
+                    a0 += wave_acc[k][lane].x;
+                    a1 += wave_acc[k][lane].y;
+                }
+            }
+            const float inv = 1.0f / lsum;
+            reinterpret_cast<uint32_t *>(a.out + row * kAttD)[lane] = lsum == 0.0f ? 0u : pack_rne(a0 * inv, a1 * inv);
+        }
+
+        int launch_merge(const char *what, const CacheArgs &a, int block_cols, hipStream_t stream)
+        {
+            if (a.splits > 1)
+            {
+                const dim3 threads(kMergeWaves * kWave);
+                if (a.rows <= kAttBlockMergeRows)
+                    cache_merge_kernel<kMergeWaves><<<dim3(static_cast<unsigned>(a.rows)), threads, 0, stream>>>(a, block_cols);
+                else
+                    cache_merge_kernel<1><<<dim3(static_cast<unsigned>(blocks_for(a.rows, kMergeWaves))), threads, 0, stream>>>(
+                        a, block_cols);
+            }
+            return check_launch(what);
+        }
+
+        template <int KW, bool E4M3, bool TREE>
+        int launch_decode(const char *what, const CacheArgs &a, int64_t B, hipStream_t stream)
+        {
+            const int64_t blocks = B * a.Hkv * a.splits;
+            if (!launch_fits(blocks, KW * kWave))
+                return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
+            cache_decode_kernel<KW, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(KW * kWave), 0, stream>>>(a);
+            return launch_merge(what, a, kAttColsPerWave, stream);
+        }
+
+        template <int CW, int KW, int HH, bool E4M3, bool TREE>
+        int launch_block(const char *what, CacheArgs a, int64_t B, hipStream_t stream)
+        {
+            constexpr int kBlockCols = 32 * CW, kThreads = CW * KW * kWave;
+            a.qblocks = static_cast<int32_t>(blocks_for(a.S * (a.Hq / a.Hkv), kBlockCols));
+            const int64_t blocks = B * a.Hkv * a.qblocks * a.splits;
+            if (!launch_fits(blocks, kThreads) || blocks > INT32_MAX)
+                return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
+            cache_block_kernel<CW, KW, HH, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(kThreads), 0, stream>>>(a);
+            return launch_merge(what, a, kBlockCols, stream);
+        }
+
+        template <bool E4M3, bool TREE>
+        int launch_fast(const char *what, const CacheArgs &a, int64_t B, const AttnSplit &p, hipStream_t stream)
+        {
+            switch (p.decode_waves)
+            {
+            case 1: return launch_decode<1, E4M3, TREE>(what, a, B, stream);
+            case 2: return launch_decode<2, E4M3, TREE>(what, a, B, stream);
+            case 4: return launch_decode<4, E4M3, TREE>(what, a, B, stream);
+            default: break;
+            }
+            switch (p.key_groups)
+            {
+            case 2: return launch_block<4, 2, 2, E4M3, TREE>(what, a, B, stream);
+            case 4: return launch_block<2, 4, 1, E4M3, TREE>(what, a, B, stream);
+            default: return launch_block<4, 1, 2, E4M3, TREE>(what, a, B, stream);
+            }
+        }
+
+        // Whether the matrix-core kernels take the call: rows and Q in 16-byte vectors, a
+        // tile's rows within 32-bit byte offsets.
+        bool fast(const CacheArgs &a, bool e4m3)
+        {
+            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) ||
+                !aligned_to(a.out, 8))
+                return false;
+            if (e4m3)
+                return aligned_to(a.scales, 2);
+            const int64_t row_limit = (INT32_MAX - 2 * kAttD) / (2 * kAttKeyTile);
+            for (const int64_t s : {a.ks0, a.ks1, a.ks2, a.vs0, a.vs1, a.vs2})
+                if (s % 8 != 0)
+                    return false;
+            return a.ks3 == 1 && a.vs3 == 1 && a.ks1 <= row_limit && a.vs1 <= row_limit;
+        }
+
         // The checks that the three calls share, in the order of the bf16
         // attention's; `strides` are K's and V's, non-negative.
         int validate(const char *what, const CacheArgs &a, int64_t B, int64_t bound)
@@ -235,10 +1295,25 @@ namespace q3k
             return Q3K_OK;
         }
 
-        int launch(const char *what, CacheArgs a, int64_t B, bool e4m3, void *, int64_t, hipStream_t stream)
+        int launch(const char *what, CacheArgs a, int64_t B, bool e4m3, void *workspace, int64_t workspace_bytes,
+                   hipStream_t stream)
         {
             a.scale = 1.0f / __builtin_sqrtf(static_cast<float>(a.D));
             a.rows = B * a.S * a.Hq;
+            if (fast(a, e4m3))
+            {
+                AttnSplit p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, true);
+                if (p.splits > 1 && (p.splits > kAttMaxSplits || workspace == nullptr || !aligned16(workspace) ||
+                                     workspace_bytes < p.bytes))
+                    p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, false);
+                a.splits = p.splits;
+                a.split_keys = p.split_keys;
+                a.part_o = static_cast<float *>(workspace);
+                a.part_ml = p.splits > 1 ? a.part_o + static_cast<int64_t>(p.splits) * a.rows * kAttD : nullptr;
+                if (a.parents != nullptr)
+                    return e4m3 ? launch_fast<true, true>(what, a, B, p, stream) : launch_fast<false, true>(what, a, B, p, stream);
+                return launch_fast<true, false>(what, a, B, p, stream);
+            }
             const int64_t blocks = blocks_for(a.rows, kBlock / kWave);
             if (!launch_fits(blocks, kBlock))
                 return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
@@ -356,7 +1431,10 @@ extern "C" int q3k_gqa_tree_attention_e4m3_bf16(const uint16_t *q, const uint8_t
     return launch(what, a, B, true, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
-extern "C" int64_t q3k_cache_attention_workspace_bytes(int64_t, int64_t, int32_t, int32_t, int32_t, int64_t)
+extern "C" int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int32_t D, int64_t cached)
 {
-    return 0;
+    if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D != q3k::kAttD || cached <= 0 || cached > INT32_MAX ||
+        S > INT64_MAX / B || B * S > INT64_MAX / Hq || B * S * Hq > INT32_MAX)
+        return 0;
+    return q3k::attention_workspace_bound(B, S, Hq, Hkv, cached);
 }

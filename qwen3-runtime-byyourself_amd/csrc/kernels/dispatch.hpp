@@ -339,13 +339,9 @@ namespace q3k
     // be cut into: a caller that sizes it once for the length of its cache never has
     // too little for a shorter context.  (The plan's own slices go up and down with the
     // length: 64 sequences of 4 / 1 heads take 4 slices at 16384 keys and 16 at 1924.)
-    // With no keys before the S positions there is no shorter context, and it is the
-    // call's own: 0 for a prefill of 2048 tokens of 16 / 8 heads, where the bound is 49 MiB.
-    inline int64_t attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
+    inline int64_t attention_workspace_bound(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
     {
         const int64_t pairs = B * Hkv, cols = S * (Hq / Hkv);
-        if (cached == S)
-            return plan_attention_split(B, S, Hq, Hkv, cached).bytes;
         int64_t most, keys; // slices, and the fewest keys of one
         if (cols <= kAttColsPerWave)
         {
@@ -365,6 +361,14 @@ namespace q3k
         for (const int64_t bound : {static_cast<int64_t>(kAttMaxSplits), blocks_for(cached, keys)})
             most = most < bound ? most : bound;
         return most < 2 ? 0 : most * B * S * Hq * (kAttHeadDim + 2) * 4;
+    }
+
+    // What q3k_gqa_attention_bf16 asks for.  With no keys before the S positions there
+    // is no shorter context, and it is the call's own: 0 for a prefill of 2048 tokens of
+    // 16 / 8 heads, where the bound is 49 MiB.
+    inline int64_t attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
+    {
+        return cached == S ? plan_attention_split(B, S, Hq, Hkv, cached).bytes : attention_workspace_bound(B, S, Hq, Hkv, cached);
     }
 
     // Which kernel merges the slices of the query rows.
@@ -424,6 +428,31 @@ namespace q3k
             p.waves = p.split.decode_waves;
         else if (p.split.key_groups == 1 && (G == 1 || G == 2 || G == 4 || G == 8 || G == 16 || G == 32))
             p.g_instance = G;
+        return p;
+    }
+
+    // ---- attention over a cache with a length for each sequence ---------------
+
+    // Key groups, waves and split of the attention over an e4m3 or a bf16 cache, for
+    // sequences of up to `cached` rows.  A row of codes is half the bytes of a bf16 one
+    // and a tile of the decode kernel 64 rows instead of 32, so with few columns the
+    // e4m3 cache is planned as a bf16 one of half the rows; with more the products
+    // bound both alike.
+    inline AttnSplit plan_cache_attention(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3,
+                                          bool can_split)
+    {
+        const int64_t most = cached > 1 ? cached : 1;
+        if (S * (Hq / Hkv) > kAttColsPerWave)
+            return plan_attention_prefill(B, S, Hq, Hkv, most > S ? most : S, can_split);
+        if (!e4m3)
+            return plan_attention_decode(B, S, Hq, Hkv, most, can_split);
+        AttnSplit p = plan_attention_decode(B, S, Hq, Hkv, (most + 1) / 2, can_split);
+        if (p.splits > 1)
+        {
+            p.split_keys *= 2;
+            p.splits = static_cast<int32_t>(blocks_for(most, p.split_keys));
+            p.bytes = static_cast<int64_t>(p.splits) * B * S * Hq * (kAttHeadDim + 2) * 4;
+        }
         return p;
     }
 } // namespace q3k
