@@ -458,7 +458,7 @@ Q3K_API int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S,
  * bytes copied unchanged: a bf16 or fp32 cache [layers, batch_cap, seq_cap,
  * Hkv, D] has heads = 1 and row_bytes of a whole position, an e4m3 cache
  * heads = Hkv and row_bytes = D, and its scales [layers, batch_cap, heads,
- * seq_cap, 2] move along (NULL: none).  B <= batch_cap.
+ * seq_cap, 2] (2-byte aligned) move along (NULL: none).  B <= batch_cap.
  */
 Q3K_API int q3k_kv_keep_path(void *key_cache, void *value_cache, uint8_t *scales,
                           int64_t layers, int64_t batch_cap, int32_t heads,

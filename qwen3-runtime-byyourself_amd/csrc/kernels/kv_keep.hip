@@ -1,27 +1,29 @@
 // Keeping the accepted path of drafted tokens, for gfx950: in every layer of a
 // KV cache, row start + path[b, i] of sequence b moves to row start + i.
 //
-// A thread owns one word of the rows of one (layer, sequence, head), K's or V's
-// (or the two scale bytes of an e4m3 cache), and moves it for the whole path,
-// kPathStep entries at a time: their loads, then their stores.  Because an entry
-// is only followed where path[b, i] >= i, a word is read before any store
-// reaches it: the stores so far went to rows below the step's first entry, and
-// every later source is at least its own index.  So rows may overlap and no
-// second buffer is needed.  What bounds it is latency for one sequence (a read
-// of the path, a read of the rows, a store) and memory for many.
+// A wave owns a few chunks of one (layer, sequence): a chunk is up to 64 words of a
+// head's K or V rows, and where a row is narrower (128 bytes of codes: 8 words) the
+// lanes hold that many entries of the path side by side.  It moves them kStep
+// entries at a time, all loads before the stores.  An entry is only followed where
+// path[b, i] >= i, so whatever is read from row i belongs to an entry at or before
+// i: its load was issued with or before that of entry i, and the store to row i
+// waits for that one.  So rows may overlap and no second buffer is needed.
+// What bounds it is latency for one sequence (the path beside its count and start, a
+// read of the rows, a store) and scattered rows of 128 bytes for many.
 #include "q3k_common.hpp"
 
 namespace q3k
 {
     namespace
     {
-        constexpr int kPathStep = 8;
-
         struct KeepShape
         {
-            int64_t items;     // layers * B * heads * words of a row (K's, V's and one for the scales)
+            int64_t waves;     // layers * B * groups
+            uint32_t groups;   // of chunks of a (layer, sequence)
+            uint32_t chunks;   // heads * 2 * chunks of a row
+            uint32_t per_row;  // chunks of a row
             uint32_t words;    // words of a row
-            uint32_t per_row;  // 2 * words, one more with scales
+            uint32_t shift;    // log2 of the lanes of a row
             uint32_t B;
             uint32_t heads;
             int64_t batch_cap;
@@ -33,77 +35,106 @@ namespace q3k
             const int32_t *counts;
         };
 
-        // Moves the word at base (rows `stride` words apart) along the path.
-        template <typename W>
-        __device__ __forceinline__ void keep_word(W *base, int64_t stride, const KeepShape &s, const int32_t *path, int64_t n,
-                                                  int64_t start)
+        // Which row an entry comes from, below 0 where it stays.  The path is read
+        // whatever the count is, so that the two are read together.
+        __device__ __forceinline__ int64_t entry_row(const KeepShape &s, const int32_t *path, int64_t i, int64_t n, int64_t start)
         {
-            for (int64_t i0 = 0; i0 < n; i0 += kPathStep)
+            const int64_t p = i < s.path_len ? path[i] : -1;
+            return i < n && p > i && start + p < s.seq_cap ? start + p : -1;
+        }
+
+        // U chunks and N entries a lane at once.
+        template <typename W, int U, int N>
+        __global__ __launch_bounds__(kBlock) void keep_path_kernel(W *__restrict__ k, W *__restrict__ v, uint16_t *__restrict__ scales,
+                                                                   KeepShape s)
+        {
+            const int64_t wave = static_cast<int64_t>(blockIdx.x) * (kBlock / kWave) +
+                                 __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+            if (wave >= s.waves)
+                return;
+            const int lane = threadIdx.x % kWave;
+            // layers, sequences and groups are below 2^31 together (checked by the launcher)
+            const uint32_t w32 = static_cast<uint32_t>(wave);
+            const uint32_t lb = w32 / s.groups, group = w32 - lb * s.groups;
+            const uint32_t layer = lb / s.B, b = lb - layer * s.B;
+            const int32_t *path = s.path + b * s.path_len;
+            const int64_t start = s.starts != nullptr ? s.starts[b] : s.start;
+            const int64_t count = s.counts != nullptr ? s.counts[b] : s.path_len;
+            const int64_t n = start < 0 ? 0 : count < s.path_len ? count : s.path_len;
+            const int64_t row0 = (static_cast<int64_t>(layer) * s.batch_cap + b) * s.heads * s.seq_cap;
+
+            const int entries = kWave >> s.shift, entry = lane >> s.shift;
+            const uint32_t sub = static_cast<uint32_t>(lane) & ((1u << s.shift) - 1u);
+            W *base[U];
+            bool have[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
             {
-                W val[kPathStep];
-                bool move[kPathStep];
+                const uint32_t c = group * U + u, row = (c / 2) / s.per_row, word = ((c / 2) % s.per_row << s.shift) + sub;
+                have[u] = c < s.chunks && word < s.words;
+                base[u] = (c % 2 == 0 ? k : v) + (row0 + row * s.seq_cap) * s.words + word;
+            }
+            for (int64_t i0 = 0; i0 < n; i0 += entries * N)
+            {
+                W val[U][N];
+                int64_t from[N];
 #pragma unroll
-                for (int u = 0; u < kPathStep; ++u)
+                for (int x = 0; x < N; ++x)
+                    from[x] = entry_row(s, path, i0 + x * entries + entry, n, start);
+#pragma unroll
+                for (int x = 0; x < N; ++x)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (have[u] && from[x] >= 0)
+                            val[u][x] = base[u][from[x] * s.words];
+#pragma unroll
+                for (int x = 0; x < N; ++x)
+#pragma unroll
+                    for (int u = 0; u < U; ++u)
+                        if (have[u] && from[x] >= 0)
+                            base[u][(start + i0 + x * entries + entry) * s.words] = val[u][x];
+            }
+            // the scale pairs: eight heads by eight entries, the heads dealt to the groups
+            if (scales == nullptr)
+                return;
+            for (uint32_t h0 = group * 8; h0 < s.heads; h0 += s.groups * 8)
+            {
+                const uint32_t h = h0 + lane / 8;
+                uint16_t *at = scales + row0 + h * s.seq_cap;
+                for (int64_t i0 = 0; i0 < n; i0 += 8)
                 {
-                    const int64_t i = i0 + u;
-                    const int64_t p = i < n ? path[i] : -1;
-                    // also false for i past the end: p is -1 there
-                    move[u] = p > i && start + p < s.seq_cap;
-                    if (move[u])
-                        val[u] = base[(start + p) * stride];
+                    const int64_t i = i0 + lane % 8, from = entry_row(s, path, i, n, start);
+                    if (h < s.heads && from >= 0)
+                        at[start + i] = at[from];
                 }
-#pragma unroll
-                for (int u = 0; u < kPathStep; ++u)
-                    if (move[u])
-                        base[(start + i0 + u) * stride] = val[u];
             }
         }
 
         template <typename W>
-        __global__ __launch_bounds__(kBlock) void keep_path_kernel(W *k, W *v, uint8_t *scales, KeepShape s)
-        {
-            const int64_t threads = static_cast<int64_t>(gridDim.x) * kBlock;
-            for (int64_t item = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x; item < s.items; item += threads)
-            {
-                const int64_t outer = item / s.per_row;
-                const uint32_t w = static_cast<uint32_t>(item - outer * s.per_row);
-                const int64_t lb = outer / s.heads;
-                const uint32_t h = static_cast<uint32_t>(outer - lb * s.heads);
-                const int64_t layer = lb / s.B;
-                const uint32_t b = static_cast<uint32_t>(lb - layer * s.B);
-                const int64_t start = s.starts != nullptr ? s.starts[b] : s.start;
-                int64_t n = s.path_len;
-                if (s.counts != nullptr)
-                    n = s.counts[b] < n ? s.counts[b] : n;
-                if (start < 0 || start >= s.seq_cap)
-                    continue;
-                const int32_t *path = s.path + b * s.path_len;
-                const int64_t row0 = ((layer * s.batch_cap + b) * s.heads + h) * s.seq_cap;
-                if (w < s.words)
-                    keep_word(k + row0 * s.words + w, s.words, s, path, n, start);
-                else if (w < 2 * s.words)
-                    keep_word(v + row0 * s.words + (w - s.words), s.words, s, path, n, start);
-                else
-                {
-                    // the two scale bytes of a row, which may lie at an odd address
-                    struct Pair
-                    {
-                        uint8_t k, v;
-                    };
-                    keep_word(reinterpret_cast<Pair *>(scales) + row0, int64_t{1}, s, path, n, start);
-                }
-            }
-        }
-
-        template <typename W>
-        void launch_keep(void *k, void *v, uint8_t *scales, KeepShape s, int64_t outer, int64_t row_bytes, hipStream_t stream)
+        int launch_keep(void *k, void *v, uint8_t *scales, KeepShape s, int64_t lb, int64_t row_bytes, hipStream_t stream)
         {
             s.words = static_cast<uint32_t>(row_bytes / static_cast<int64_t>(sizeof(W)));
-            s.per_row = 2 * s.words + (scales != nullptr ? 1u : 0u);
-            s.items = outer * s.per_row;
-            const int64_t blocks = blocks_for(s.items, kBlock), most = int64_t{1} << 22;
-            keep_path_kernel<W><<<dim3(static_cast<unsigned>(blocks < most ? blocks : most)), dim3(kBlock), 0, stream>>>(
-                static_cast<W *>(k), static_cast<W *>(v), scales, s);
+            while ((1u << s.shift) < s.words && (1u << s.shift) < static_cast<uint32_t>(kWave))
+                ++s.shift;
+            s.per_row = static_cast<uint32_t>(blocks_for(s.words, int64_t{1} << s.shift));
+            // rows of a wave's width or more: one chunk and eight entries a wave; narrower
+            // ones: the entries lie side by side, and eight chunks are moved at once
+            const bool wide = s.shift == 6;
+            const int64_t chunks = static_cast<int64_t>(s.heads) * 2 * s.per_row;
+            const int64_t groups = wide ? chunks : blocks_for(chunks, 8);
+            if (chunks > INT32_MAX || groups > INT32_MAX / lb || !launch_fits(blocks_for(lb * groups, kBlock / kWave), kBlock))
+                return set_error(Q3K_ERR_OVERFLOW, "KV keep grid is too large");
+            s.chunks = static_cast<uint32_t>(chunks);
+            s.groups = static_cast<uint32_t>(groups);
+            s.waves = lb * groups;
+            const dim3 grid(static_cast<unsigned>(blocks_for(s.waves, kBlock / kWave))), block(kBlock);
+            W *kw = static_cast<W *>(k), *vw = static_cast<W *>(v);
+            uint16_t *sc = reinterpret_cast<uint16_t *>(scales);
+            if (wide)
+                keep_path_kernel<W, 1, 8><<<grid, block, 0, stream>>>(kw, vw, sc, s);
+            else
+                keep_path_kernel<W, 8, 1><<<grid, block, 0, stream>>>(kw, vw, sc, s);
+            return check_launch("kv_keep_path");
         }
     } // namespace
 } // namespace q3k
@@ -135,6 +166,8 @@ extern "C" int q3k_kv_keep_path(void *key_cache, void *value_cache, uint8_t *sca
         return set_error(Q3K_ERR_INVALID_ARGUMENT, "KV keep received a null pointer");
     if (!aligned_to(path, 4) || !aligned_to(starts, 4) || !aligned_to(counts, 4))
         return set_error(Q3K_ERR_INVALID_ARGUMENT, "KV keep index pointers must be 4-byte aligned");
+    if (!aligned_to(scales, 2))
+        return set_error(Q3K_ERR_INVALID_ARGUMENT, "KV keep scales must be 2-byte aligned");
     KeepShape s{};
     s.B = static_cast<uint32_t>(B);
     s.heads = static_cast<uint32_t>(heads);
@@ -145,17 +178,17 @@ extern "C" int q3k_kv_keep_path(void *key_cache, void *value_cache, uint8_t *sca
     s.path_len = path_len;
     s.starts = starts;
     s.counts = counts;
-    const int64_t outer = layers * B * heads;
+    if (layers > INT32_MAX / B)
+        return set_error(Q3K_ERR_OVERFLOW, "KV keep grid is too large");
+    const int64_t lb = layers * B;
     const hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     const auto fits = [&](int64_t w) {
         return row_bytes % w == 0 && aligned_to(key_cache, static_cast<uintptr_t>(w)) &&
                aligned_to(value_cache, static_cast<uintptr_t>(w));
     };
     if (fits(16))
-        launch_keep<Vec8>(key_cache, value_cache, scales, s, outer, row_bytes, st);
-    else if (fits(4))
-        launch_keep<uint32_t>(key_cache, value_cache, scales, s, outer, row_bytes, st);
-    else
-        launch_keep<uint8_t>(key_cache, value_cache, scales, s, outer, row_bytes, st);
-    return check_launch("kv_keep_path");
+        return launch_keep<Vec8>(key_cache, value_cache, scales, s, lb, row_bytes, st);
+    if (fits(4))
+        return launch_keep<uint32_t>(key_cache, value_cache, scales, s, lb, row_bytes, st);
+    return launch_keep<uint8_t>(key_cache, value_cache, scales, s, lb, row_bytes, st);
 }

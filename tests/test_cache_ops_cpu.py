@@ -115,7 +115,7 @@ def test_keep_refusals(q3k):
     _expect(keep, OverflowError, OV, 2, 4, 1, 16, 2**31, 2, 0, 4)
     for name in ("kc", "vc", "path"):
         _expect(keep, ValueError, IA, 2, 4, 1, 16, 64, 2, 0, 4, **{name: None})
-    for kw in ({"path": F + 1}, {"starts": F + 2}, {"counts": F + 3}):
+    for kw in ({"path": F + 1}, {"starts": F + 2}, {"counts": F + 3}, {"sc": F + 1}):
         _expect(keep, ValueError, IA, 2, 4, 1, 16, 64, 2, 0, 4, **kw)
     keep(0, 4, 1, 16, 64, 2, 0, 4, kc=None)
     keep(2, 4, 1, 16, 64, 0, 0, 4, kc=None)

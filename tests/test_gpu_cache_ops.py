@@ -363,7 +363,7 @@ def test_keep_path(q3k, hip, heads, row, dtype, scaled, offset):
     path[3, 2:6] = [0, -1, 9, 9]                        # up, negative, the same node twice
     counts = np.array([n, 7, n, n, n], np.int32)
     for given_counts in (True, False):
-        bufs = [Guarded(hip, a, offset=offset) for a in (k, v)] + [Guarded(hip, s, offset=offset % 2) if scaled else None]
+        bufs = [Guarded(hip, a, offset=offset) for a in (k, v)] + [Guarded(hip, s) if scaled else None]
         bp, bs, bc = _up(hip, path, starts, counts)
         q3k.kv_keep_path(*bufs, L, cap_b, heads, seq, row, B, 0, bp, n, starts=bs, counts=bc if given_counts else None)
         hip.synchronize()
