@@ -43,6 +43,23 @@ namespace q3k
             return i < n && p > i && start + p < s.seq_cap ? start + p : -1;
         }
 
+        template <typename W>
+        __device__ __forceinline__ W load_word(const W *p)
+        {
+            if constexpr (sizeof(W) == 16)
+                return load8<true>(p);
+            else
+                return *p;
+        }
+        template <typename W>
+        __device__ __forceinline__ void store_word(W *p, const W &w)
+        {
+            if constexpr (sizeof(W) == 16)
+                store8<kStoreStream>(p, w);
+            else
+                *p = w;
+        }
+
         // U chunks and N entries a lane at once.
         template <typename W, int U, int N>
         __global__ __launch_bounds__(kBlock) void keep_path_kernel(W *__restrict__ k, W *__restrict__ v, uint16_t *__restrict__ scales,
@@ -86,13 +103,13 @@ namespace q3k
 #pragma unroll
                     for (int u = 0; u < U; ++u)
                         if (have[u] && from[x] >= 0)
-                            val[u][x] = base[u][from[x] * s.words];
+                            val[u][x] = load_word(base[u] + from[x] * s.words);
 #pragma unroll
                 for (int x = 0; x < N; ++x)
 #pragma unroll
                     for (int u = 0; u < U; ++u)
                         if (have[u] && from[x] >= 0)
-                            base[u][(start + i0 + x * entries + entry) * s.words] = val[u][x];
+                            store_word(base[u] + (start + i0 + x * entries + entry) * s.words, val[u][x]);
             }
             // the scale pairs: eight heads by eight entries, the heads dealt to the groups
             if (scales == nullptr)
