@@ -131,25 +131,50 @@ namespace q3k
                 scales[2 * at + l] = static_cast<uint8_t>(l == 0 ? sk : sv);
         }
 
+        // kReadPositions positions of a sequence a lane, all their codes before the stores:
+        // a head's positions lie together in the cache.  Groups of G lanes run over the heads
+        // first, so that a wave's stores cover whole positions.
+        constexpr int kReadPositions = 4;
+
         template <int G>
         __global__ __launch_bounds__(kBlock) void read_rows_kernel(const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc,
                                                                    const uint8_t *__restrict__ scales, Vec8 *__restrict__ k,
-                                                                   Vec8 *__restrict__ v, E4m3Shape s)
+                                                                   Vec8 *__restrict__ v, E4m3Shape s, uint32_t steps)
         {
-            const uint32_t row = blockIdx.x * (kBlock / G) + threadIdx.x / G;
-            if (row >= s.rows)
+            // unit: (sequence, step of positions, head)
+            const uint32_t unit = blockIdx.x * (kBlock / G) + threadIdx.x / G;
+            const uint32_t bp = unit / s.Hkv, h = unit - bp * s.Hkv;
+            const uint32_t b = bp / steps, p0 = (bp - b * steps) * kReadPositions;
+            if (b >= s.rows / (s.S * s.Hkv))
                 return;
             const uint32_t l = threadIdx.x % G;
-            const uint32_t token = row / s.Hkv, h = row - token * s.Hkv;
-            const uint32_t b = token / s.S;
-            const int64_t pos = s.start + (token - b * s.S);
-            if (s.starts != nullptr && pos >= s.starts[b])
-                return;
-            const int64_t at = cache_row(s, b, h, pos);
-            const uint2 ck = reinterpret_cast<const uint2 *>(kc)[at * G + l], cv = reinterpret_cast<const uint2 *>(vc)[at * G + l];
-            const float sk = e4m3_scale(scales[2 * at]), sv = e4m3_scale(scales[2 * at + 1]);
-            store8<kStoreStream>(k + static_cast<int64_t>(row) * G + l, decode8(ck, sk));
-            store8<kStoreStream>(v + static_cast<int64_t>(row) * G + l, decode8(cv, sv));
+            // positions of this sequence that are read, counted from start
+            int64_t n = s.S;
+            if (s.starts != nullptr)
+                n = s.starts[b] - s.start < n ? s.starts[b] - s.start : n;
+            const int64_t at = cache_row(s, b, h, s.start + p0);
+            const uint2 *kp = reinterpret_cast<const uint2 *>(kc) + at * G + l, *vp = reinterpret_cast<const uint2 *>(vc) + at * G + l;
+            const uint8_t *sp = scales + 2 * at;
+            uint2 ck[kReadPositions], cv[kReadPositions];
+            uint32_t sk[kReadPositions], sv[kReadPositions];
+#pragma unroll
+            for (int u = 0; u < kReadPositions; ++u)
+                if (p0 + u < n)
+                {
+                    ck[u] = kp[u * G];
+                    cv[u] = vp[u * G];
+                    sk[u] = sp[2 * u];
+                    sv[u] = sp[2 * u + 1];
+                }
+            const int64_t row0 = (static_cast<int64_t>(b) * s.S + p0) * s.Hkv + h;
+#pragma unroll
+            for (int u = 0; u < kReadPositions; ++u)
+                if (p0 + u < n)
+                {
+                    const int64_t out = (row0 + static_cast<int64_t>(u) * s.Hkv) * G + l;
+                    store8<kStoreStream>(k + out, decode8(ck[u], e4m3_scale(sk[u])));
+                    store8<kStoreStream>(v + out, decode8(cv[u], e4m3_scale(sv[u])));
+                }
         }
 
         // Any head_dim and alignment: a wave a row, K then V.
@@ -293,12 +318,14 @@ extern "C" int q3k_kv_read_e4m3_bf16(const uint8_t *k_codes, const uint8_t *v_co
     Vec8 *k = reinterpret_cast<Vec8 *>(key), *v = reinterpret_cast<Vec8 *>(value);
     const dim3 block(kBlock);
     const int lanes = row_lanes(s, aligned16(key) && aligned16(value) && aligned_to(k_codes, 8) && aligned_to(v_codes, 8));
-    const dim3 grid(lanes == 0 ? generic_grid(s) : static_cast<unsigned>(blocks_for(s.rows, kBlock / lanes)));
+    const int64_t steps = blocks_for(count, kReadPositions);
+    const dim3 grid(lanes == 0 ? generic_grid(s) : static_cast<unsigned>(blocks_for(B * steps * Hkv, kBlock / lanes)));
+    const uint32_t st32 = static_cast<uint32_t>(steps);
     switch (lanes)
     {
-    case 8: read_rows_kernel<8><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
-    case 16: read_rows_kernel<16><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
-    case 32: read_rows_kernel<32><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
+    case 8: read_rows_kernel<8><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
+    case 16: read_rows_kernel<16><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
+    case 32: read_rows_kernel<32><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
     default: read_generic_kernel<<<grid, block, 0, st>>>(k_codes, v_codes, scales, key, value, s); break;
     }
     return check_launch("kv_read_e4m3");
