@@ -59,6 +59,8 @@ namespace q3k
             int32_t D;
             float scale;
             int64_t rows;
+            int32_t B;
+            bool ordered; // blocks take the sequences longest first
             // the fast kernels: query blocks of a pair, slices of split_keys rows, their
             // results (unnormalised O^T [splits, rows, D], reference max and sum
             // [splits, rows, 2])
@@ -86,6 +88,42 @@ namespace q3k
             const int64_t n = a.lengths != nullptr ? a.lengths[b] : a.cached;
             bad = n < 0 || n > a.cached || (a.parents != nullptr && n > 0 && n < a.S);
             return bad ? 0 : static_cast<int32_t>(n);
+        }
+
+        // Sequences of different lengths: blocks take them longest first, so that what
+        // starts last is short; and while all blocks are on the GPU at once, 256 to a round,
+        // every second round goes the other way, so that a CU's blocks are a long and a
+        // short one.  (64 sequences of 1024 to 4096 rows, 8 KV heads, in 512 blocks of two
+        // waves: X us, Y in the order given.)  Of more than 64 sequences each 64 are ordered
+        // among themselves.
+
+        // The unit that block i of `units` takes, units ordered longest first.
+        __device__ __forceinline__ int32_t long_and_short(int32_t i, int32_t units, int32_t resident)
+        {
+            constexpr int32_t kCus = 256;
+            const int32_t round = i / kCus;
+            if (units > resident || round % 2 == 0)
+                return i;
+            const int32_t last = units < (round + 1) * kCus ? units - 1 : (round + 1) * kCus - 1;
+            return last - (i - round * kCus);
+        }
+
+        // The sequence that comes `rank`-th by length; the whole wave calls it.
+        __device__ __forceinline__ int32_t sequence_at(const CacheArgs &a, int32_t rank, int lane)
+        {
+            if (!a.ordered)
+                return rank;
+            const int32_t first = rank / kWave * kWave;
+            // equal lengths in the order given; lanes past the last sequence come last
+            const int32_t n = first + lane < a.B ? a.lengths[first + lane] : -1;
+            uint32_t before = 0;
+#pragma unroll
+            for (int i = 0; i < kWave; ++i)
+            {
+                const int32_t other = __builtin_amdgcn_readlane(n, i);
+                before += (other > n) || (other == n && i < lane) ? 1u : 0u;
+            }
+            return first + static_cast<int32_t>(__builtin_ctzll(__ballot(before == static_cast<uint32_t>(rank - first))));
         }
 
         // Walks up from node t and calls visit(u) for the node and each ancestor.
@@ -288,32 +326,33 @@ namespace q3k
         __device__ __forceinline__ int k_slot8(int r, int c) { return c ^ ((r >> 1) & 7); }
         __device__ __forceinline__ int v_slot8(int r, int c) { return c ^ ((r & 2) | ((r >> 1) & 4)); }
 
-        // S^T of the 64 keys of a tile of codes; scale[hh]: that of key 32 hh + li.  A
+        // S^T of the 32 HH keys of a tile of codes; scale[hh]: that of key 32 hh + li.  A
         // lane's 16 codes of chunk 2 c + lg are the dims of Q fragments 2 c and 2 c + 1
         // (load_q orders them so).
-        template <typename Next>
+        template <int HH>
         __device__ __forceinline__ void qk_codes(const unsigned char *k_lds, const bf16x8_t (&qf)[kAttD / 16], int li, int lg,
-                                                 const float (&scale)[2], f32x16_t (&sacc)[2], Next next)
+                                                 const float (&scale)[HH], f32x16_t (&sacc)[HH])
         {
             auto read = [&](int c, int hh) __attribute__((always_inline)) {
                 return *reinterpret_cast<const uint4 *>(k_lds + (32 * hh + li) * kAttD + 16 * k_slot8(li, 2 * c + lg));
             };
-            sacc[0] = f32x16_t{};
-            sacc[1] = f32x16_t{};
-            uint4 codes[2][2] = {{read(0, 0), read(0, 1)}, {}};
+            uint4 codes[2][HH];
+#pragma unroll
+            for (int hh = 0; hh < HH; ++hh)
+            {
+                sacc[hh] = f32x16_t{};
+                codes[0][hh] = read(0, hh);
+            }
 #pragma unroll
             for (int c = 0; c < kAttD / 32; ++c)
             {
                 if (c + 1 < kAttD / 32)
-                {
-                    codes[(c + 1) % 2][0] = read(c + 1, 0);
-                    codes[(c + 1) % 2][1] = read(c + 1, 1);
-                }
-                else
-                    next();
+#pragma unroll
+                    for (int hh = 0; hh < HH; ++hh)
+                        codes[(c + 1) % 2][hh] = read(c + 1, hh);
                 __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
 #pragma unroll
-                for (int hh = 0; hh < 2; ++hh)
+                for (int hh = 0; hh < HH; ++hh)
                 {
                     const uint4 w = codes[c % 2][hh];
                     sacc[hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.x, w.y), scale[hh])), qf[2 * c],
@@ -343,17 +382,19 @@ namespace q3k
             return make_uint2(static_cast<uint32_t>(c.x), static_cast<uint32_t>(c.y));
         }
 
+        template <int HH>
         __device__ __forceinline__ void pv_codes(const unsigned char *v_lds, const int (&v_off)[kAttD / 32],
-                                                 const bf16x8_t (&phi)[2][2], const bf16x8_t (&plo)[2][2], f32x16_t (&o)[kAttD / 32])
+                                                 const bf16x8_t (&phi)[HH][2], const bf16x8_t (&plo)[HH][2],
+                                                 f32x16_t (&o)[kAttD / 32])
         {
             uint2 vq[kAhead + 1];
 #pragma unroll
             for (int x = 0; x < kAhead; ++x)
                 vq[x] = read_v8(v_lds, v_off, x);
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < 8 * HH; ++i)
             {
-                if (i + kAhead < 16)
+                if (i + kAhead < 8 * HH)
                     vq[(i + kAhead) % (kAhead + 1)] = read_v8(v_lds, v_off, i + kAhead);
                 __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
                 const int dt = i % 4, hh = i / 8, mm = (i / 4) % 2;
@@ -517,10 +558,10 @@ namespace q3k
         // streams its own tiles (8 KiB of K and of V: 64 keys of codes or 32 of bf16)
         // through two K and two V buffers with no barrier, as the causal bf16 attention
         // does; the scales of a tile's rows come along, a word a key.
-        template <int KW, bool E4M3, bool TREE>
-        __global__ __launch_bounds__(KW *kWave) void cache_decode_kernel(CacheArgs a)
+        template <int KW, int HH, bool E4M3, bool TREE>
+        __global__ __launch_bounds__(KW *kWave, E4M3 && HH == 1 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
         {
-            constexpr int RB = E4M3 ? kAttD : kRowBytes, HH = E4M3 ? 2 : 1, kKeys = 32 * HH, kTileBytes = kKeys * RB;
+            constexpr int RB = E4M3 ? kAttD : kRowBytes, kKeys = 32 * HH, kTileBytes = kKeys * RB;
             using St = Staging<1, kKeys, RB>;
             constexpr int kL = St::kLoads, kS = E4M3 ? 1 : 0;
             __shared__ __attribute__((aligned(16))) unsigned char k_a[KW * kTileBytes];
@@ -535,9 +576,10 @@ namespace q3k
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
             // slices of a pair side by side
-            const int sp = static_cast<int>(blockIdx.x) % a.splits, pair = static_cast<int>(blockIdx.x) / a.splits;
-            const int kvh = pair % a.Hkv;
-            const int64_t b = pair / a.Hkv;
+            const int32_t unit = long_and_short(static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), 1024 / KW);
+            const int32_t sp = unit % a.splits, pair = unit / a.splits;
+            const int32_t kvh = pair % a.Hkv;
+            const int64_t b = sequence_at(a, pair / a.Hkv, lane);
             const int32_t S = static_cast<int32_t>(a.S);
             const int g = a.Hq / a.Hkv;
             bool bad;
@@ -586,8 +628,8 @@ namespace q3k
                 {
                     const int last = n_keys - 1 - tile * kKeys;
                     __builtin_amdgcn_raw_ptr_buffer_load_lds(tile_rsrc(sbase + 2 * static_cast<int64_t>(tile) * kKeys),
-                                                             (lds_void_t *)(sbuf + kw * kWave), 2, 2 * (lane < last ? lane : last), 0,
-                                                             0, 0);
+                                                             (lds_void_t *)(sbuf + kw * kWave), 2,
+                                                             2 * (lane % kKeys < last ? lane % kKeys : last), 0, 0, 0);
                 }
                 load_tile_rows<1, kKeys, RB>(tile, buf + kw * kTileBytes, kbase, kstride, n_keys, 0, lane, k_voff, kslot);
             };
@@ -637,9 +679,15 @@ namespace q3k
                     const uint32_t vbyte = pair_bytes >> 8;
                     vs[lane] = e4m3_scale(vbyte < 254u ? vbyte : 254u);
                     const uint32_t ks = (pair_bytes & 255u) << 23;
-                    const auto halves = __builtin_amdgcn_permlane32_swap(ks, ks, false, false);
-                    const float k_scale[2] = {__uint_as_float(halves[0]), __uint_as_float(halves[1])};
-                    qk_codes(k_lds, qf, li, lg, k_scale, sacc, []() __attribute__((always_inline)) {});
+                    float k_scale[HH];
+                    k_scale[0] = __uint_as_float(ks);
+                    if constexpr (HH == 2)
+                    {
+                        const auto halves = __builtin_amdgcn_permlane32_swap(ks, ks, false, false);
+                        k_scale[0] = __uint_as_float(halves[0]);
+                        k_scale[1] = __uint_as_float(halves[1]);
+                    }
+                    qk_codes<HH>(k_lds, qf, li, lg, k_scale, sacc);
                 }
                 else
                     qk_tile<HH>(k_lds, qf, li, lg, sacc, [](int) __attribute__((always_inline)) {});
@@ -702,7 +750,7 @@ namespace q3k
                         seen, phi, plo, o);
                 }
                 else if constexpr (E4M3)
-                    pv_codes(v_lds, v_off, phi, plo, o);
+                    pv_codes<HH>(v_lds, v_off, phi, plo, o);
                 else
                 {
                     bf16x8_t vq[kAhead + 1];
@@ -784,14 +832,31 @@ namespace q3k
             const int cw = wave % CW, kw = wave / CW;
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
-            // the pair runs fastest (one XCD holds a pair's K and V), the query blocks of a
-            // slice longest first, slices outermost
-            const int pairs = static_cast<int>(gridDim.x) / (a.qblocks * a.splits);
-            const int pair = static_cast<int>(blockIdx.x) % pairs;
-            const int rest = static_cast<int>(blockIdx.x) / pairs;
-            const int sp = rest / a.qblocks, qb = a.qblocks - 1 - rest % a.qblocks;
-            const int kvh = pair % a.Hkv;
-            const int64_t b = pair / a.Hkv;
+            // KV heads run fastest, so that with a multiple of 8 of them the blocks of a pair
+            // meet on one XCD, whose L2 holds its K and V.  A tree's query blocks are equally
+            // long: sequences outermost, longest first.  Causal ones differ: slices
+            // outermost, then the query blocks, longest first, then the sequences.
+            int32_t sp, qb, kvh, rank;
+            if constexpr (TREE)
+            {
+                int32_t unit = long_and_short(static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), KW == 1 ? 512 : 256);
+                kvh = unit % a.Hkv;
+                unit /= a.Hkv;
+                qb = unit % a.qblocks;
+                unit /= a.qblocks;
+                sp = unit % a.splits;
+                rank = unit / a.splits;
+            }
+            else
+            {
+                const int32_t pairs = static_cast<int32_t>(gridDim.x) / (a.qblocks * a.splits);
+                const int32_t pair = static_cast<int32_t>(blockIdx.x) % pairs, rest = static_cast<int32_t>(blockIdx.x) / pairs;
+                sp = rest / a.qblocks;
+                qb = a.qblocks - 1 - rest % a.qblocks;
+                kvh = pair % a.Hkv;
+                rank = pair / a.Hkv;
+            }
+            const int64_t b = sequence_at(a, rank, lane);
             const int32_t S = static_cast<int32_t>(a.S);
             const int32_t n_cols = S * g;
             const int32_t block_col = qb * kBlockCols;
@@ -1183,10 +1248,11 @@ namespace q3k
         template <int KW, bool E4M3, bool TREE>
         int launch_decode(const char *what, const CacheArgs &a, int64_t B, hipStream_t stream)
         {
+            constexpr int kDecodeHalves = 1;
             const int64_t blocks = B * a.Hkv * a.splits;
-            if (!launch_fits(blocks, KW * kWave))
+            if (!launch_fits(blocks, KW * kWave) || blocks > INT32_MAX)
                 return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
-            cache_decode_kernel<KW, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(KW * kWave), 0, stream>>>(a);
+            cache_decode_kernel<KW, kDecodeHalves, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(KW * kWave), 0, stream>>>(a);
             return launch_merge(what, a, kAttColsPerWave, stream);
         }
 
@@ -1224,7 +1290,8 @@ namespace q3k
         // tile's rows within 32-bit byte offsets.
         bool fast(const CacheArgs &a, bool e4m3)
         {
-            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) ||
+            // (tile ends are counted in 32 bits)
+            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || a.cached > INT32_MAX - 4 * kAttKeyTile || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) ||
                 !aligned_to(a.out, 8))
                 return false;
             if (e4m3)
@@ -1306,6 +1373,8 @@ namespace q3k
                 if (p.splits > 1 && (p.splits > kAttMaxSplits || workspace == nullptr || !aligned16(workspace) ||
                                      workspace_bytes < p.bytes))
                     p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, false);
+                a.B = static_cast<int32_t>(B);
+                a.ordered = a.lengths != nullptr && B > 1 && (p.splits == 1 || p.decode_waves == 0);
                 a.splits = p.splits;
                 a.split_keys = p.split_keys;
                 a.part_o = static_cast<float *>(workspace);
