@@ -13,9 +13,8 @@
 // S^T = K Q^T, online softmax, O^T += V^T P^T, keys in tiles, up to 32 (position,
 // head) columns to a wave.
 //   Few columns (at most 32 to a (sequence, KV head): decode, small trees): the
-//   block's waves divide the keys and stream their own tiles through LDS.  A tile
-//   of the e4m3 cache is 64 keys of 128 bytes; its codes stay 8 bits wide until a
-//   fragment is in registers: K's with ds_read_b128, 16 dims of a key, converted
+//   block's waves divide the keys and stream their own tiles of 32 keys through
+//   LDS.  Codes stay 8 bits wide until a fragment is in registers: K's with ds_read_b128, 16 dims of a key, converted
 //   to two bf16 fragments with the key's scale (a lane holds one key, so the scale
 //   is one register); V's with the 8-bit transpose read, 8 keys of a dim, converted
 //   without a scale, which is multiplied into the weights instead (there a lane
@@ -300,18 +299,20 @@ namespace q3k
             return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u;
         }
 
-        // The bit of element r of a lane's S^T half in its window.
-        __device__ __forceinline__ uint32_t element_bit(int r, int lg) { return 1u << (8 * (r / 4) + 4 * lg + r % 4); }
-
+        // Element r of a lane's S^T half is key 8 (r / 4) + 4 lg + r % 4: the window is moved
+        // by 4 lg once, and each element tests a bit that is a constant.
         template <int HH>
         __device__ __forceinline__ void mask_scores(f32x16_t (&sacc)[HH], const uint32_t (&seen)[HH], int lg)
         {
 #pragma unroll
             for (int hh = 0; hh < HH; ++hh)
+            {
+                const uint32_t w = seen[hh] >> (4 * lg);
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if ((seen[hh] & element_bit(r, lg)) == 0)
+                    if ((w >> (8 * (r / 4) + r % 4) & 1u) == 0)
                         sacc[hh][r] = -__builtin_huge_valf();
+            }
         }
 
         // ---- products over e4m3 tiles ------------------------------------------------
@@ -326,41 +327,28 @@ namespace q3k
         __device__ __forceinline__ int k_slot8(int r, int c) { return c ^ ((r >> 1) & 7); }
         __device__ __forceinline__ int v_slot8(int r, int c) { return c ^ ((r & 2) | ((r >> 1) & 4)); }
 
-        // S^T of the 32 HH keys of a tile of codes; scale[hh]: that of key 32 hh + li.  A
-        // lane's 16 codes of chunk 2 c + lg are the dims of Q fragments 2 c and 2 c + 1
-        // (load_q orders them so).
-        template <int HH>
-        __device__ __forceinline__ void qk_codes(const unsigned char *k_lds, const bf16x8_t (&qf)[kAttD / 16], int li, int lg,
-                                                 const float (&scale)[HH], f32x16_t (&sacc)[HH])
+        // S^T of the 32 keys of a tile of codes; scale: that of key li.  A lane's 16 codes of
+        // chunk 2 c + lg are the dims of Q fragments 2 c and 2 c + 1 (load_q orders them so).
+        __device__ __forceinline__ f32x16_t qk_codes(const unsigned char *k_lds, const bf16x8_t (&qf)[kAttD / 16], int li, int lg,
+                                                     float scale)
         {
-            auto read = [&](int c, int hh) __attribute__((always_inline)) {
-                return *reinterpret_cast<const uint4 *>(k_lds + (32 * hh + li) * kAttD + 16 * k_slot8(li, 2 * c + lg));
+            auto read = [&](int c) __attribute__((always_inline)) {
+                return *reinterpret_cast<const uint4 *>(k_lds + li * kAttD + 16 * k_slot8(li, 2 * c + lg));
             };
-            uint4 codes[2][HH];
-#pragma unroll
-            for (int hh = 0; hh < HH; ++hh)
-            {
-                sacc[hh] = f32x16_t{};
-                codes[0][hh] = read(0, hh);
-            }
+            f32x16_t sacc = f32x16_t{};
+            uint4 codes[2] = {read(0), {}};
 #pragma unroll
             for (int c = 0; c < kAttD / 32; ++c)
             {
                 if (c + 1 < kAttD / 32)
-#pragma unroll
-                    for (int hh = 0; hh < HH; ++hh)
-                        codes[(c + 1) % 2][hh] = read(c + 1, hh);
+                    codes[(c + 1) % 2] = read(c + 1);
                 __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
-#pragma unroll
-                for (int hh = 0; hh < HH; ++hh)
-                {
-                    const uint4 w = codes[c % 2][hh];
-                    sacc[hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.x, w.y), scale[hh])), qf[2 * c],
-                                                                       sacc[hh], 0, 0, 0);
-                    sacc[hh] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.z, w.w), scale[hh])),
-                                                                       qf[2 * c + 1], sacc[hh], 0, 0, 0);
-                }
+                const uint4 w = codes[c % 2];
+                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.x, w.y), scale)), qf[2 * c], sacc, 0, 0, 0);
+                sacc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf8(decode8(make_uint2(w.z, w.w), scale)), qf[2 * c + 1], sacc, 0,
+                                                               0, 0);
             }
+            return sacc;
         }
 
         // Per-lane LDS offsets of V's 8-bit transpose reads: lanes 2 i, 2 i + 1 of each 16
@@ -382,25 +370,23 @@ namespace q3k
             return make_uint2(static_cast<uint32_t>(c.x), static_cast<uint32_t>(c.y));
         }
 
-        template <int HH>
-        __device__ __forceinline__ void pv_codes(const unsigned char *v_lds, const int (&v_off)[kAttD / 32],
-                                                 const bf16x8_t (&phi)[HH][2], const bf16x8_t (&plo)[HH][2],
-                                                 f32x16_t (&o)[kAttD / 32])
+        __device__ __forceinline__ void pv_codes(const unsigned char *v_lds, const int (&v_off)[kAttD / 32], const bf16x8_t (&phi)[1][2],
+                                                 const bf16x8_t (&plo)[1][2], f32x16_t (&o)[kAttD / 32])
         {
             uint2 vq[kAhead + 1];
 #pragma unroll
             for (int x = 0; x < kAhead; ++x)
                 vq[x] = read_v8(v_lds, v_off, x);
 #pragma unroll
-            for (int i = 0; i < 8 * HH; ++i)
+            for (int i = 0; i < 8; ++i)
             {
-                if (i + kAhead < 8 * HH)
+                if (i + kAhead < 8)
                     vq[(i + kAhead) % (kAhead + 1)] = read_v8(v_lds, v_off, i + kAhead);
                 __builtin_amdgcn_sched_barrier(0); // keep the reads ahead of these MFMAs
-                const int dt = i % 4, hh = i / 8, mm = (i / 4) % 2;
+                const int dt = i % 4, mm = i / 4;
                 const bf16x8_t v = as_bf8(decode8(vq[i % (kAhead + 1)], 1.0f));
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, phi[hh][mm], o[dt], 0, 0, 0);
-                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, plo[hh][mm], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, phi[0][mm], o[dt], 0, 0, 0);
+                o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(v, plo[0][mm], o[dt], 0, 0, 0);
             }
         }
 
@@ -555,13 +541,19 @@ namespace q3k
 
         // At most 32 columns to a (sequence, KV head): one wave holds them all, the
         // block's KW waves divide the keys and share nothing until the merge.  Each
-        // streams its own tiles (8 KiB of K and of V: 64 keys of codes or 32 of bf16)
+        // streams its own tiles of 32 keys (8 KiB of bf16 K and of V, 4 KiB of codes)
         // through two K and two V buffers with no barrier, as the causal bf16 attention
         // does; the scales of a tile's rows come along, a word a key.
-        template <int KW, int HH, bool E4M3, bool TREE>
-        __global__ __launch_bounds__(KW *kWave, E4M3 && HH == 1 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
+        // What bounds it is memory for many sequences, one wave's chain of tiles for few.  A
+        // tile of codes is half the bytes of a bf16 one at the same work, so two waves go on
+        // a SIMD (64 KiB of LDS a block, at most 256 registers) and one's conversions and
+        // softmax run beside the other's: with 64-key tiles and one wave a SIMD 64 ragged
+        // sequences of up to 4096 rows took 73.3 us against 69.2, their trees of 5 nodes 51.3
+        // against 39.2.
+        template <int KW, bool E4M3, bool TREE>
+        __global__ __launch_bounds__(KW *kWave, E4M3 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
         {
-            constexpr int RB = E4M3 ? kAttD : kRowBytes, kKeys = 32 * HH, kTileBytes = kKeys * RB;
+            constexpr int RB = E4M3 ? kAttD : kRowBytes, kKeys = kCacheDecodeTile, kTileBytes = kKeys * RB;
             using St = Staging<1, kKeys, RB>;
             constexpr int kL = St::kLoads, kS = E4M3 ? 1 : 0;
             __shared__ __attribute__((aligned(16))) unsigned char k_a[KW * kTileBytes];
@@ -669,63 +661,48 @@ namespace q3k
                     wait_loads<3 * kL + kS>();
                 else
                     wait_loads<kL>();
-                f32x16_t sacc[HH];
+                f32x16_t sacc[1];
                 if constexpr (E4M3)
                 {
-                    // lane i has the scales of key i: K's go to the lanes that hold the key's
-                    // codes, i and i + 32 (one swap gives both halves), V's to LDS.  A row
-                    // past the end may hold any byte; 254 keeps its scale finite.
+                    // lane i has the scales of key i % 32: K's for the codes it reads of that key,
+                    // V's go to LDS.  A row past the end may hold any byte; 254 keeps its scale
+                    // finite.
                     const uint32_t pair_bytes = sb[kw * kWave + lane];
                     const uint32_t vbyte = pair_bytes >> 8;
                     vs[lane] = e4m3_scale(vbyte < 254u ? vbyte : 254u);
-                    const uint32_t ks = (pair_bytes & 255u) << 23;
-                    float k_scale[HH];
-                    k_scale[0] = __uint_as_float(ks);
-                    if constexpr (HH == 2)
-                    {
-                        const auto halves = __builtin_amdgcn_permlane32_swap(ks, ks, false, false);
-                        k_scale[0] = __uint_as_float(halves[0]);
-                        k_scale[1] = __uint_as_float(halves[1]);
-                    }
-                    qk_codes<HH>(k_lds, qf, li, lg, k_scale, sacc);
+                    sacc[0] = qk_codes(k_lds, qf, li, lg, e4m3_scale(pair_bytes & 255u));
                 }
                 else
-                    qk_tile<HH>(k_lds, qf, li, lg, sacc, [](int) __attribute__((always_inline)) {});
+                    qk_tile<1>(k_lds, qf, li, lg, sacc, [](int) __attribute__((always_inline)) {});
                 wait_loads<63>();
                 if (j + 2 < mine)
                     load_k(j + 2, kb, sb);
                 const int32_t key0 = (first + KW * j) * kKeys;
                 const bool masked = key0 + kKeys > all_seen;
-                uint32_t seen[HH];
+                uint32_t seen[1];
                 if (masked)
                 {
-#pragma unroll
-                    for (int hh = 0; hh < HH; ++hh)
-                    {
-                        if constexpr (TREE)
-                            seen[hh] = tree_window(tree.mask[s_row], key0 + 32 * hh - context);
-                        else
-                            seen[hh] = causal_window(key0 + 32 * hh, context + s_row);
-                    }
-                    mask_scores<HH>(sacc, seen, lg);
+                    if constexpr (TREE)
+                        seen[0] = tree_window(tree.mask[s_row], key0 - context);
+                    else
+                        seen[0] = causal_window(key0, context + s_row);
+                    mask_scores<1>(sacc, seen, lg);
                 }
-                bf16x8_t phi[HH][2], plo[HH][2];
+                bf16x8_t phi[1][2], plo[1][2];
                 float alpha;
                 if constexpr (E4M3)
                 {
-                    float4 w[HH][4];
+                    float4 w[4];
 #pragma unroll
-                    for (int hh = 0; hh < HH; ++hh)
-#pragma unroll
-                        for (int q4 = 0; q4 < 4; ++q4)
-                            w[hh][q4] = *reinterpret_cast<const float4 *>(vs + 32 * hh + 8 * q4 + 4 * lg);
-                    alpha = softmax_tile<HH>(sacc, scale2, m, l, phi, plo, [&](float p, int hh, int r) __attribute__((always_inline)) {
-                        const float4 &x = w[hh][r / 4];
+                    for (int q4 = 0; q4 < 4; ++q4)
+                        w[q4] = *reinterpret_cast<const float4 *>(vs + 8 * q4 + 4 * lg);
+                    alpha = softmax_tile<1>(sacc, scale2, m, l, phi, plo, [&](float p, int, int r) __attribute__((always_inline)) {
+                        const float4 &x = w[r / 4];
                         return p * (r % 4 == 0 ? x.x : r % 4 == 1 ? x.y : r % 4 == 2 ? x.z : x.w);
                     });
                 }
                 else
-                    alpha = softmax_tile<HH>(sacc, scale2, m, l, phi, plo);
+                    alpha = softmax_tile<1>(sacc, scale2, m, l, phi, plo);
                 rescale(o, alpha);
                 // V(j), then K(j + 1), V(j + 1), K(j + 2)
                 if (j + 2 < mine)
@@ -737,7 +714,7 @@ namespace q3k
                 // one query sees every row up to its own, and past it only repeats of that row
                 if (masked && S > 1 && has_nonfinite<E4M3>(v_lds, kTileBytes, lane))
                 {
-                    pv_careful<HH>(
+                    pv_careful<1>(
                         [&](int i) __attribute__((always_inline)) {
                             if constexpr (E4M3)
                                 return as_bf8(decode8(read_v8(v_lds, v_off, i), 1.0f));
@@ -750,14 +727,14 @@ namespace q3k
                         seen, phi, plo, o);
                 }
                 else if constexpr (E4M3)
-                    pv_codes<HH>(v_lds, v_off, phi, plo, o);
+                    pv_codes(v_lds, v_off, phi, plo, o);
                 else
                 {
                     bf16x8_t vq[kAhead + 1];
 #pragma unroll
                     for (int x = 0; x < kAhead; ++x)
                         vq[x] = read_v(v_lds, v_off, x);
-                    pv_tile<HH>(v_lds, v_off, phi, plo, o, vq);
+                    pv_tile<1>(v_lds, v_off, phi, plo, o, vq);
                 }
                 wait_loads<63>();
                 if (j + 2 < mine)
@@ -834,7 +811,8 @@ namespace q3k
             const int li = lane % 32, lg = lane / 32;
             // KV heads run fastest, so that with a multiple of 8 of them the blocks of a pair
             // meet on one XCD, whose L2 holds its K and V.  A tree's query blocks are equally
-            // long: sequences outermost, longest first.  Causal ones differ: slices
+            // long: sequences outermost, longest first; but a last block of fewer columns is
+            // lighter, and those come after all others.  Causal ones differ: slices
             // outermost, then the query blocks, longest first, then the sequences.
             int32_t sp, qb, kvh, rank;
             if constexpr (TREE)
@@ -842,8 +820,10 @@ namespace q3k
                 int32_t unit = long_and_short(static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), KW == 1 ? 512 : 256);
                 kvh = unit % a.Hkv;
                 unit /= a.Hkv;
-                qb = unit % a.qblocks;
-                unit /= a.qblocks;
+                const int32_t whole = static_cast<int32_t>(a.S) * g / kBlockCols; // query blocks of all their columns
+                const int32_t light = unit - a.B * a.splits * whole;
+                qb = light >= 0 ? whole : unit % whole;
+                unit = light >= 0 ? light : unit / whole;
                 sp = unit % a.splits;
                 rank = unit / a.splits;
             }
@@ -1137,109 +1117,149 @@ namespace q3k
 
         // ---- merging slices ---------------------------------------------------------------
 
-        // WPR waves to a query row: lane i of each reads slice i's reference max and sum,
-        // wave w the unnormalised O^T of slices w, w + WPR, ... (all loads of a round
-        // before any is used); weights 2^(m_i - max m), then sum w O / sum w l.  A row
-        // whose query block fits one slice is already done.
-        constexpr int kMergeWaves = 4;
-        constexpr int kMergeRound = kAttMaxSplits / kMergeWaves;
-
-        template <int WPR>
-        __global__ __launch_bounds__(kMergeWaves *kWave) void cache_merge_kernel(CacheArgs a, int32_t block_cols)
+        // How many slices hold a query row's keys; 0: its query block wrote the result.
+        // With several positions a row takes the slices its own keys reach (in the others of
+        // its query block all its scores are masked).
+        __device__ __forceinline__ int row_slices(const CacheArgs &a, int64_t row, int32_t block_cols)
         {
-            static_assert(WPR == 1 || WPR == kMergeWaves, "waves per row");
-            __shared__ float2 wave_acc[kMergeWaves][kWave];
-            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-            const int lane = threadIdx.x % kWave;
-            const int part = WPR == 1 ? 0 : wave;
-            const int64_t row = WPR == 1 ? static_cast<int64_t>(blockIdx.x) * kMergeWaves + wave : blockIdx.x;
-            if (row >= a.rows)
-                return; // whole waves, and with one row a wave no barrier below
             const uint32_t r32 = static_cast<uint32_t>(row), hq = static_cast<uint32_t>(a.Hq), S = static_cast<uint32_t>(a.S);
             const uint32_t bs = r32 / hq, h = r32 - bs * hq, b = bs / S;
             const int32_t s = static_cast<int32_t>(bs - b * S);
             bool bad;
             const int32_t n = sequence_rows(a, b, bad);
             if (n == 0)
-                return;
-            int32_t own = n; // rows this query's slices reach
+                return 0;
+            int32_t own = n, block = n; // rows that this query's slices and its block's reach
             if (a.parents == nullptr)
             {
                 const int32_t g = a.Hq / a.Hkv, col = s * g + static_cast<int32_t>(h) % g;
                 const int64_t last = ((static_cast<int64_t>(col) / block_cols + 1) * block_cols - 1) / g;
                 const int32_t s_last = last < a.S ? static_cast<int32_t>(last) : static_cast<int32_t>(a.S) - 1;
                 own = n - static_cast<int32_t>(a.S) + s + 1;
-                if (own + s_last - s <= a.split_keys)
-                    return;
+                block = own + s_last - s;
             }
-            else if (n <= a.split_keys)
+            return block <= a.split_keys ? 0 : own <= 0 ? 1 : (own - 1) / a.split_keys + 1;
+        }
+
+        // Few rows, many slices: a block of four waves a row.  Lane i of each wave reads
+        // slice i's reference max and sum, wave w the unnormalised O^T of slices w, w + 4,
+        // ..., all before any is used; weights 2^(m_i - max m), then sum w O / sum w l.
+        constexpr int kMergeWaves = 4;
+        constexpr int kMergeRound = kAttMaxSplits / kMergeWaves;
+
+        __global__ __launch_bounds__(kMergeWaves *kWave) void cache_merge_block_kernel(CacheArgs a, int32_t block_cols)
+        {
+            __shared__ float2 wave_acc[kMergeWaves][kWave];
+            const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+            const int lane = threadIdx.x % kWave;
+            const int64_t row = blockIdx.x;
+            const int slices = row_slices(a, row, block_cols);
+            if (slices == 0)
                 return;
-            const int splits = own <= 0 ? 1 : (own - 1) / a.split_keys + 1;
             float2 ml = make_float2(-__builtin_huge_valf(), 0.0f);
-            if (lane < splits)
+            if (lane < slices)
                 ml = reinterpret_cast<const float2 *>(a.part_ml)[static_cast<int64_t>(lane) * a.rows + row];
-            float a0 = 0.0f, a1 = 0.0f, w = 0.0f;
-            auto round = [&](int s0) __attribute__((always_inline)) {
-                float2 v[kMergeRound];
+            float2 v[kMergeRound];
 #pragma unroll
-                for (int u = 0; u < kMergeRound; ++u)
-                {
-                    const int sp = s0 + part + WPR * u;
-                    if (sp < splits)
-                        v[u] = reinterpret_cast<const float2 *>(a.part_o + (static_cast<int64_t>(sp) * a.rows + row) * kAttD)[lane];
-                }
-                if (s0 == 0)
-                {
-                    float mx = ml.x;
-#pragma unroll
-                    for (int off = kWave / 2; off > 0; off /= 2)
-                        mx = fmaxf(mx, __shfl_xor(mx, off, kWave));
-                    mx = mx == -__builtin_huge_valf() ? 0.0f : mx;
-                    w = lane < splits ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
-                }
-#pragma unroll
-                for (int u = 0; u < kMergeRound; ++u)
-                {
-                    const int sp = s0 + part + WPR * u;
-                    if (sp < splits)
-                    {
-                        const float ws = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), sp));
-                        a0 += ws * v[u].x;
-                        a1 += ws * v[u].y;
-                    }
-                }
-            };
-            round(0);
-            if constexpr (WPR == 1)
-                for (int s0 = kMergeRound; s0 < splits; s0 += kMergeRound)
-                    round(s0);
-            const float lsum = group_sum<kWave>(w * ml.y);
-            if constexpr (WPR > 1)
+            for (int u = 0; u < kMergeRound; ++u)
             {
-                wave_acc[wave][lane] = make_float2(a0, a1);
-                __syncthreads();
-                if (part != 0)
-                    return;
+                const int i = wave + kMergeWaves * u;
+                if (i < slices)
+                    v[u] = reinterpret_cast<const float2 *>(a.part_o + (static_cast<int64_t>(i) * a.rows + row) * kAttD)[lane];
+            }
+            float mx = ml.x;
 #pragma unroll
-                for (int k = 1; k < WPR; ++k)
+            for (int off = kWave / 2; off > 0; off /= 2)
+                mx = fmaxf(mx, __shfl_xor(mx, off, kWave));
+            mx = mx == -__builtin_huge_valf() ? 0.0f : mx;
+            const float w = lane < slices ? __builtin_amdgcn_exp2f(ml.x - mx) : 0.0f;
+            float a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+            for (int u = 0; u < kMergeRound; ++u)
+            {
+                const int i = wave + kMergeWaves * u;
+                if (i < slices)
                 {
-                    a0 += wave_acc[k][lane].x;
-                    a1 += wave_acc[k][lane].y;
+                    const float wi = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), i));
+                    a0 += wi * v[u].x;
+                    a1 += wi * v[u].y;
                 }
+            }
+            const float lsum = group_sum<kWave>(w * ml.y);
+            wave_acc[wave][lane] = make_float2(a0, a1);
+            __syncthreads();
+            if (wave != 0)
+                return;
+#pragma unroll
+            for (int k = 1; k < kMergeWaves; ++k)
+            {
+                a0 += wave_acc[k][lane].x;
+                a1 += wave_acc[k][lane].y;
             }
             const float inv = 1.0f / lsum;
             reinterpret_cast<uint32_t *>(a.out + row * kAttD)[lane] = lsum == 0.0f ? 0u : pack_rne(a0 * inv, a1 * inv);
+        }
+
+        // Many rows: 16 lanes a row, 8 dims a lane, four slices at a time; every lane works
+        // the weights out for itself, so nothing is exchanged.
+        constexpr int kMergeSlices = 4;
+        constexpr int kMergeRows = kBlock / 16;
+
+        __global__ __launch_bounds__(kBlock) void cache_merge_rows_kernel(CacheArgs a, int32_t block_cols)
+        {
+            const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeRows + threadIdx.x / 16;
+            if (row >= a.rows)
+                return;
+            const int slices = row_slices(a, row, block_cols), d = 8 * (threadIdx.x % 16);
+            if (slices == 0)
+                return;
+            float mx = -__builtin_huge_valf(), lsum = 0.0f, acc[8] = {};
+            for (int i0 = 0; i0 < slices; i0 += kMergeSlices)
+            {
+                float2 ml[kMergeSlices];
+                float4 v[kMergeSlices][2];
+#pragma unroll
+                for (int u = 0; u < kMergeSlices; ++u)
+                    if (i0 + u < slices)
+                    {
+                        const int64_t at = static_cast<int64_t>(i0 + u) * a.rows + row;
+                        ml[u] = reinterpret_cast<const float2 *>(a.part_ml)[at];
+                        const float4 *po = reinterpret_cast<const float4 *>(a.part_o + at * kAttD + d);
+                        v[u][0] = po[0];
+                        v[u][1] = po[1];
+                    }
+#pragma unroll
+                for (int u = 0; u < kMergeSlices; ++u)
+                    if (i0 + u < slices)
+                    {
+                        const float m = fmaxf(mx, ml[u].x), m_use = m == -__builtin_huge_valf() ? 0.0f : m;
+                        const float w0 = __builtin_amdgcn_exp2f(mx - m_use), w = __builtin_amdgcn_exp2f(ml[u].x - m_use);
+                        lsum = lsum * w0 + ml[u].y * w;
+                        const float e[8] = {v[u][0].x, v[u][0].y, v[u][0].z, v[u][0].w, v[u][1].x, v[u][1].y, v[u][1].z, v[u][1].w};
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+                            acc[j] = acc[j] * w0 + e[j] * w;
+                        mx = m;
+                    }
+            }
+            const float inv = 1.0f / lsum;
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                w[j] = lsum == 0.0f ? 0u : pack_rne(acc[2 * j] * inv, acc[2 * j + 1] * inv);
+            uint2 *o = reinterpret_cast<uint2 *>(a.out + row * kAttD + d); // out is 8-byte aligned
+            o[0] = make_uint2(w[0], w[1]);
+            o[1] = make_uint2(w[2], w[3]);
         }
 
         int launch_merge(const char *what, const CacheArgs &a, int block_cols, hipStream_t stream)
         {
             if (a.splits > 1)
             {
-                const dim3 threads(kMergeWaves * kWave);
                 if (a.rows <= kAttBlockMergeRows)
-                    cache_merge_kernel<kMergeWaves><<<dim3(static_cast<unsigned>(a.rows)), threads, 0, stream>>>(a, block_cols);
+                    cache_merge_block_kernel<<<dim3(static_cast<unsigned>(a.rows)), dim3(kMergeWaves * kWave), 0, stream>>>(a, block_cols);
                 else
-                    cache_merge_kernel<1><<<dim3(static_cast<unsigned>(blocks_for(a.rows, kMergeWaves))), threads, 0, stream>>>(
+                    cache_merge_rows_kernel<<<dim3(static_cast<unsigned>(blocks_for(a.rows, kMergeRows))), dim3(kBlock), 0, stream>>>(
                         a, block_cols);
             }
             return check_launch(what);
@@ -1248,11 +1268,10 @@ namespace q3k
         template <int KW, bool E4M3, bool TREE>
         int launch_decode(const char *what, const CacheArgs &a, int64_t B, hipStream_t stream)
         {
-            constexpr int kDecodeHalves = 1;
             const int64_t blocks = B * a.Hkv * a.splits;
             if (!launch_fits(blocks, KW * kWave) || blocks > INT32_MAX)
                 return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
-            cache_decode_kernel<KW, kDecodeHalves, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(KW * kWave), 0, stream>>>(a);
+            cache_decode_kernel<KW, E4M3, TREE><<<dim3(static_cast<unsigned>(blocks)), dim3(KW * kWave), 0, stream>>>(a);
             return launch_merge(what, a, kAttColsPerWave, stream);
         }
 
@@ -1269,21 +1288,13 @@ namespace q3k
         }
 
         template <bool E4M3, bool TREE>
-        int launch_fast(const char *what, const CacheArgs &a, int64_t B, const AttnSplit &p, hipStream_t stream)
+        int launch_fast(const char *what, const CacheArgs &a, int64_t B, const CacheAttnPlan &p, hipStream_t stream)
         {
-            switch (p.decode_waves)
-            {
-            case 1: return launch_decode<1, E4M3, TREE>(what, a, B, stream);
-            case 2: return launch_decode<2, E4M3, TREE>(what, a, B, stream);
-            case 4: return launch_decode<4, E4M3, TREE>(what, a, B, stream);
-            default: break;
-            }
-            switch (p.key_groups)
-            {
-            case 2: return launch_block<4, 2, 2, E4M3, TREE>(what, a, B, stream);
-            case 4: return launch_block<2, 4, 1, E4M3, TREE>(what, a, B, stream);
-            default: return launch_block<4, 1, 2, E4M3, TREE>(what, a, B, stream);
-            }
+            if (p.decode_waves > 0)
+                return p.decode_waves == 1 ? launch_decode<1, E4M3, TREE>(what, a, B, stream)
+                                           : launch_decode<4, E4M3, TREE>(what, a, B, stream);
+            return p.key_groups == 1 ? launch_block<4, 1, 2, E4M3, TREE>(what, a, B, stream)
+                                     : launch_block<2, 4, 1, E4M3, TREE>(what, a, B, stream);
         }
 
         // Whether the matrix-core kernels take the call: rows and Q in 16-byte vectors, a
@@ -1369,17 +1380,17 @@ namespace q3k
             a.rows = B * a.S * a.Hq;
             if (fast(a, e4m3))
             {
-                AttnSplit p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, true);
-                if (p.splits > 1 && (p.splits > kAttMaxSplits || workspace == nullptr || !aligned16(workspace) ||
-                                     workspace_bytes < p.bytes))
-                    p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, false);
+                const bool tree = a.parents != nullptr, ragged = a.lengths != nullptr;
+                CacheAttnPlan p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, tree, ragged, true);
+                if (p.bytes > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < p.bytes))
+                    p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, tree, ragged, false);
                 a.B = static_cast<int32_t>(B);
-                a.ordered = a.lengths != nullptr && B > 1 && (p.splits == 1 || p.decode_waves == 0);
+                a.ordered = ragged && B > 1 && (p.splits == 1 || p.decode_waves == 0);
                 a.splits = p.splits;
                 a.split_keys = p.split_keys;
                 a.part_o = static_cast<float *>(workspace);
                 a.part_ml = p.splits > 1 ? a.part_o + static_cast<int64_t>(p.splits) * a.rows * kAttD : nullptr;
-                if (a.parents != nullptr)
+                if (tree)
                     return e4m3 ? launch_fast<true, true>(what, a, B, p, stream) : launch_fast<false, true>(what, a, B, p, stream);
                 return launch_fast<true, false>(what, a, B, p, stream);
             }
@@ -1505,5 +1516,5 @@ extern "C" int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S, int
     if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D != q3k::kAttD || cached <= 0 || cached > INT32_MAX ||
         S > INT64_MAX / B || B * S > INT64_MAX / Hq || B * S * Hq > INT32_MAX)
         return 0;
-    return q3k::attention_workspace_bound(B, S, Hq, Hkv, cached);
+    return q3k::cache_attention_workspace_bytes(B, S, Hq, Hkv, cached);
 }

@@ -339,9 +339,13 @@ namespace q3k
     // be cut into: a caller that sizes it once for the length of its cache never has
     // too little for a shorter context.  (The plan's own slices go up and down with the
     // length: 64 sequences of 4 / 1 heads take 4 slices at 16384 keys and 16 at 1924.)
-    inline int64_t attention_workspace_bound(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
+    // With no keys before the S positions there is no shorter context, and it is the
+    // call's own: 0 for a prefill of 2048 tokens of 16 / 8 heads, where the bound is 49 MiB.
+    inline int64_t attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
     {
         const int64_t pairs = B * Hkv, cols = S * (Hq / Hkv);
+        if (cached == S)
+            return plan_attention_split(B, S, Hq, Hkv, cached).bytes;
         int64_t most, keys; // slices, and the fewest keys of one
         if (cols <= kAttColsPerWave)
         {
@@ -361,14 +365,6 @@ namespace q3k
         for (const int64_t bound : {static_cast<int64_t>(kAttMaxSplits), blocks_for(cached, keys)})
             most = most < bound ? most : bound;
         return most < 2 ? 0 : most * B * S * Hq * (kAttHeadDim + 2) * 4;
-    }
-
-    // What q3k_gqa_attention_bf16 asks for.  With no keys before the S positions there
-    // is no shorter context, and it is the call's own: 0 for a prefill of 2048 tokens of
-    // 16 / 8 heads, where the bound is 49 MiB.
-    inline int64_t attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
-    {
-        return cached == S ? plan_attention_split(B, S, Hq, Hkv, cached).bytes : attention_workspace_bound(B, S, Hq, Hkv, cached);
     }
 
     // Which kernel merges the slices of the query rows.
@@ -433,26 +429,185 @@ namespace q3k
 
     // ---- attention over a cache with a length for each sequence ---------------
 
-    // Key groups, waves and split of the attention over an e4m3 or a bf16 cache, for
-    // sequences of up to `cached` rows.  A row of codes is half the bytes of a bf16 one
-    // and a tile of the decode kernel 64 rows instead of 32, so with few columns the
-    // e4m3 cache is planned as a bf16 one of half the rows; with more the products
-    // bound both alike.
-    inline AttnSplit plan_cache_attention(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3,
-                                          bool can_split)
+    struct CacheAttnPlan
+    {
+        int32_t decode_waves = 0; // waves of a decode block (1 or 4); 0: the block kernel
+        int32_t key_groups = 1;   // block kernel: groups of waves that divide the keys (1 or 4)
+        int32_t splits = 1;       // slices of split_keys rows
+        int32_t split_keys = INT32_MAX;
+        int64_t bytes = 0;        // workspace of the slices' fp32 O^T, maxima and sums; 0: splits == 1
+    };
+
+    // Most blocks that cutting the keys may make.
+    constexpr int64_t kCacheMaxBlocks = 2048;
+    constexpr int32_t kCacheDecodeTile = 32; // rows of a decode wave's tile
+    constexpr int32_t kCacheBlockTile = 128; // slices of the block kernels are whole tiles of both
+    // What a call expects of sequences whose lengths the host does not know, as a share of
+    // the longest: of the decode kernel's time, and of the block kernels'.
+    constexpr double kRaggedDecode = 0.85, kRaggedBlock = 0.9;
+
+    inline constexpr double cache_row_bytes(bool e4m3) { return e4m3 ? 2.0 * (kAttHeadDim + 1) : 4.0 * kAttHeadDim; }
+
+    // Estimated time in us of the decode kernel in blocks of four waves and slices of
+    // split_keys rows (>= cached: whole).  A wave takes 1.7 us a tile of codes and 1.4 us a
+    // tile of bf16 rows on a busy chip, with two blocks on a CU (e4m3) 1.85 times that; all
+    // CUs read 5.1 TB/s together and one 31 GB/s; start and end take 2.7 us, another round
+    // of blocks 1.9 us, the merge 3.2 us and its bytes.  Constants fitted to 357 shapes of 1
+    // to 64 sequences, 150 to 32000 rows, 1 to 32 columns, cut into 1 to 64 slices: the
+    // slices taken so are 1.0% slower than the best of each on average, 18% at worst.
+    inline double cache_decode_us(int64_t pairs, int64_t cols, int64_t cached, bool e4m3, bool ragged, int64_t split_keys)
+    {
+        const double share = ragged ? kRaggedDecode : 1.0;
+        const int64_t keys = split_keys < cached ? split_keys : cached, slices = blocks_for(cached, keys);
+        const double blocks = static_cast<double>(pairs * slices), slots = e4m3 ? 512.0 : 256.0;
+        const double live = ragged && slices > 1 ? blocks * share : blocks;
+        const double step = (e4m3 ? 1.7 : 1.4) * (e4m3 && live > 256.0 ? 1.85 : 1.0);
+        double rounds = live / slots;
+        rounds = rounds <= 1.0 ? 1.0 : rounds < 2.5 ? static_cast<double>(static_cast<int64_t>(rounds + 0.999999)) : rounds + 0.5;
+        double us = step * static_cast<double>(blocks_for(blocks_for(keys, kCacheDecodeTile), 4)) * rounds;
+        if (ragged && slices == 1 && rounds > 1.0)
+            us *= 0.5 * (1.0 + share);
+        const double bytes = static_cast<double>(pairs) * static_cast<double>(cached) * share * cache_row_bytes(e4m3);
+        const double busy = live < 256.0 ? live : 256.0;
+        us = us > bytes / 5.1e6 ? us : bytes / 5.1e6;
+        us = us > bytes / (busy * 31.0e3) ? us : bytes / (busy * 31.0e3);
+        us += 2.7 + 1.9 * (rounds - 1.0);
+        if (slices > 1)
+            us += 3.2 + 0.01 * static_cast<double>(slices) + live * static_cast<double>(cols) * (2.0 * (kAttHeadDim + 2) * 4) / 3.0e6;
+        return us;
+    }
+
+    inline CacheAttnPlan plan_cache_decode(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool ragged,
+                                           bool can_split)
+    {
+        const int64_t pairs = B * Hkv, cols = S * (Hq / Hkv);
+        CacheAttnPlan p;
+        p.decode_waves = cached <= kCacheDecodeTile ? 1 : 4; // one tile: nothing to divide
+        if (!can_split)
+            return p;
+        double best = cache_decode_us(pairs, cols, cached, e4m3, ragged, cached);
+        for (const int slices : {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64})
+        {
+            if (slices > kAttMaxSplits || slices > kCacheMaxBlocks / pairs)
+                break;
+            const int64_t keys = blocks_for(blocks_for(cached, slices), kCacheDecodeTile) * kCacheDecodeTile;
+            if (keys >= cached || keys < 2 * kCacheDecodeTile)
+                continue;
+            const double us = cache_decode_us(pairs, cols, cached, e4m3, ragged, keys);
+            if (us >= best)
+                continue;
+            best = us;
+            p.split_keys = static_cast<int32_t>(keys);
+            p.splits = static_cast<int32_t>(blocks_for(cached, keys));
+        }
+        if (p.splits > 1)
+            p.bytes = p.splits * B * S * Hq * (kAttHeadDim + 2) * 4;
+        return p;
+    }
+
+    // Estimated time in us of the block kernels, 128 columns and one key group or 64 columns
+    // and four.  A 64-key tile takes a block alone on its CU 1.85 us (0.84 with four groups)
+    // and 1.0 us (1.25) of CU time where blocks queue or share a CU; a query block that is
+    // not full costs 0.35 of a full one and its columns' part of the rest; start and end 5.2
+    // us (4.2).  Causal query blocks see between cached - S and cached rows.  Fitted to 400
+    // shapes of 1 to 64 sequences and 12 to 400 queries or nodes: 1.1% slower than the best
+    // of the one to twenty forms of each on average, 36% at worst (4 trees of 130 nodes).
+    inline double cache_block_us(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool tree, bool ragged,
+                                 int key_groups, int64_t split_keys)
+    {
+        const int32_t G = Hq / Hkv, block_cols = attn_block_cols(key_groups);
+        const int64_t pairs = B * Hkv, cols = S * G, qblocks = blocks_for(cols, block_cols);
+        const double share = ragged ? kRaggedBlock : 1.0, rows = static_cast<double>(cached);
+        const double alone = key_groups == 1 ? 1.85 : 0.84, busy = key_groups == 1 ? 1.0 : 1.25;
+        double mean = 1.0;
+        if (!tree)
+        {
+            const int64_t positions = blocks_for(block_cols, G) < S ? blocks_for(block_cols, G) : S;
+            mean = 0.5 * (static_cast<double>(cached - S + positions) + rows) / rows;
+        }
+        const int64_t keys = split_keys < cached ? split_keys : cached, slices = blocks_for(cached, keys);
+        const double longest = alone * static_cast<double>(blocks_for(keys, 64));
+        double weight = static_cast<double>(cols / block_cols);
+        if (cols % block_cols != 0)
+            weight += 0.35 + 0.65 * static_cast<double>(cols % block_cols) / block_cols;
+        const double per_cu = static_cast<double>(pairs) * weight * rows * share * mean / 64.0 / 256.0;
+        double blocks = static_cast<double>(pairs * qblocks);
+        if (slices > 1)
+        {
+            const double n = static_cast<double>(slices) * share * mean + (ragged || !tree ? 0.5 : 0.0);
+            blocks *= n > 1.0 ? n : 1.0;
+        }
+        double us = longest;
+        if (blocks > 256.0)
+        {
+            double queued = per_cu * busy + 0.35 * longest;
+            if (key_groups == 1 && blocks <= 512.0)
+            {
+                const double both = (blocks / 256.0) * (longest / alone * busy) * (0.5 + 0.5 * share);
+                queued = both > per_cu * busy ? both : per_cu * busy;
+            }
+            us = us > queued ? us : queued;
+        }
+        const double rounds = blocks / (key_groups == 1 ? 512.0 : 256.0);
+        us += (key_groups == 1 ? 5.2 : 4.2) * (rounds <= 1.0 ? 1.0 : rounds + 0.5);
+        const double read = static_cast<double>(pairs) * rows * share * cache_row_bytes(e4m3) / 5.0e6;
+        us = us > read ? us : read;
+        if (slices > 1)
+            us += 3.0 + static_cast<double>(B * S * Hq * slices) * share * (2.0 * (kAttHeadDim + 2) * 4) / 5.6e6;
+        return us;
+    }
+
+    inline CacheAttnPlan plan_cache_block(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool tree,
+                                          bool ragged, bool can_split)
+    {
+        CacheAttnPlan p;
+        double best = -1.0;
+        for (const int key_groups : {1, 4})
+        {
+            const int64_t blocks = B * Hkv * blocks_for(S * (Hq / Hkv), attn_block_cols(key_groups));
+            for (const int slices : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48})
+            {
+                if (slices > 1 && (!can_split || slices > kCacheMaxBlocks / blocks))
+                    break;
+                const int64_t keys = blocks_for(blocks_for(cached, slices), kCacheBlockTile) * kCacheBlockTile;
+                if (slices > 1 && keys >= cached)
+                    continue;
+                const double us = cache_block_us(B, S, Hq, Hkv, cached, e4m3, tree, ragged, key_groups, slices > 1 ? keys : cached);
+                if (best >= 0.0 && us >= best)
+                    continue;
+                best = us;
+                p.key_groups = key_groups;
+                p.splits = slices > 1 ? static_cast<int32_t>(blocks_for(cached, keys)) : 1;
+                p.split_keys = slices > 1 ? static_cast<int32_t>(keys) : INT32_MAX;
+            }
+        }
+        if (p.splits > 1)
+            p.bytes = p.splits * B * S * Hq * (kAttHeadDim + 2) * 4;
+        return p;
+    }
+
+    // The attention over an e4m3 or a bf16 cache of sequences of up to `cached` rows;
+    // ragged: of lengths that the host does not know.
+    inline CacheAttnPlan plan_cache_attention(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool tree,
+                                              bool ragged, bool can_split)
     {
         const int64_t most = cached > 1 ? cached : 1;
-        if (S * (Hq / Hkv) > kAttColsPerWave)
-            return plan_attention_prefill(B, S, Hq, Hkv, most > S ? most : S, can_split);
-        if (!e4m3)
-            return plan_attention_decode(B, S, Hq, Hkv, most, can_split);
-        AttnSplit p = plan_attention_decode(B, S, Hq, Hkv, (most + 1) / 2, can_split);
-        if (p.splits > 1)
-        {
-            p.split_keys *= 2;
-            p.splits = static_cast<int32_t>(blocks_for(most, p.split_keys));
-            p.bytes = static_cast<int64_t>(p.splits) * B * S * Hq * (kAttHeadDim + 2) * 4;
-        }
-        return p;
+        if (S * (Hq / Hkv) <= kAttColsPerWave)
+            return plan_cache_decode(B, S, Hq, Hkv, most, e4m3, ragged, can_split);
+        return plan_cache_block(B, S, Hq, Hkv, most > S ? most : S, e4m3, tree, ragged, can_split);
+    }
+
+    // Workspace of the most slices that a call of these B, S and heads over up to `cached`
+    // rows may be cut into.
+    inline int64_t cache_attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached)
+    {
+        const int64_t pairs = B * Hkv, cols = S * (Hq / Hkv);
+        const bool decode = cols <= kAttColsPerWave;
+        const int64_t blocks = decode ? pairs : pairs * blocks_for(cols, attn_block_cols(1));
+        const int64_t rows = cached > S ? cached : S;
+        int64_t most = kCacheMaxBlocks / blocks;
+        for (const int64_t bound : {static_cast<int64_t>(kAttMaxSplits), blocks_for(rows, decode ? 2 * kCacheDecodeTile : kCacheBlockTile)})
+            most = most < bound ? most : bound;
+        return most < 2 ? 0 : most * B * S * Hq * (kAttHeadDim + 2) * 4;
     }
 } // namespace q3k
