@@ -2,7 +2,8 @@
 
 // Element types of the runtime's tensors.  Contract pinned by the reference's
 // tests/unit/core_metadata_test.cpp:41-54 (its src/core is absent from the
-// snapshot): dtype_size 4/2/4, dtype_name "float32"/"bfloat16"/"int32".
+// snapshot): dtype_size 4/2/4, dtype_name "float32"/"bfloat16"/"int32".  The
+// 8-bit types are this library's own.
 
 #include <cstddef>
 #include <string_view>
@@ -14,6 +15,8 @@ namespace qwen3
         Float32,
         BFloat16,
         Int32,
+        Float8E4M3, // OCP e4m3: the codes of an 8-bit KV cache
+        ScaleE8M0,  // an exponent byte s standing for 2^(s - 127): their scales
     };
 
     [[nodiscard]] std::size_t dtype_size(DType dtype);

@@ -32,6 +32,16 @@ namespace qwen3
         // start_position must equal that layer's cached length.
         void append(std::int32_t layer_index, std::int64_t start_position, const Tensor &key, const Tensor &value);
 
+        // Keeps the accepted tokens of a drafted tree (ops::tree_attention) that
+        // was appended to every layer at start_position: in each layer, row
+        // start_position + path[b, i] of sequence b moves to row start_position
+        // + i, and every layer's length becomes start_position + accepted.
+        // path: Int32 [batch, accepted] on the cache's GPU, increasing nodes of
+        // each sequence (a node is never moved up: an entry path[b, i] < i
+        // leaves its row).  Needs one length in all layers, and accepted <= the
+        // rows since start_position.
+        void keep_path(std::int64_t start_position, const Tensor &path);
+
         // Logical reset: lengths to 0, batch size unset; memory is not cleared.
         void reset() noexcept;
 

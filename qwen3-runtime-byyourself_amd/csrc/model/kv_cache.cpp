@@ -4,6 +4,7 @@
 #include "qwen3/model/kv_cache.h"
 
 #include "../ops/ops_common.hpp"
+#include "kept_path.hpp"
 
 #include <algorithm>
 #include <stdexcept>
@@ -110,6 +111,20 @@ namespace qwen3
                                  target.sequence, row_bytes, max_sequence_length_, start_position, stream);
         });
         commit_append(layer_index, start_position, target);
+    }
+
+    void KvCache::keep_path(std::int64_t start_position, const Tensor &path)
+    {
+        const std::int64_t accepted =
+            detail::check_kept_path(cached_lengths_, active_batch_size_, device_, start_position, path);
+        const std::int64_t row_bytes =
+            static_cast<std::int64_t>(num_key_value_heads_) * head_dim_ * static_cast<std::int64_t>(dtype_size(dtype_));
+        ops::detail::launch_on(device_, [&](q3k_stream_t stream) {
+            return q3k_kv_keep_path(key_storage_.data(), value_storage_.data(), nullptr, num_layers_, max_batch_size_, 1,
+                                    max_sequence_length_, row_bytes, active_batch_size_, start_position,
+                                    static_cast<const int32_t *>(path.data()), accepted, nullptr, nullptr, stream);
+        });
+        std::fill(cached_lengths_.begin(), cached_lengths_.end(), start_position + accepted);
     }
 
     void KvCache::reset() noexcept
