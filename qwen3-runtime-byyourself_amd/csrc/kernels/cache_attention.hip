@@ -113,8 +113,10 @@ namespace q3k
             if (!a.ordered)
                 return rank;
             const int32_t first = rank / kWave * kWave;
-            // equal lengths in the order given; lanes past the last sequence come last
-            const int32_t n = first + lane < a.B ? a.lengths[first + lane] : -1;
+            // equal lengths in the order given; lanes past the last sequence come last, also
+            // behind lengths below 0, which are errors but have a place
+            const int32_t length = first + lane < a.B ? a.lengths[first + lane] : 0;
+            const int32_t n = first + lane < a.B ? (length > 0 ? length : 0) : -1;
             uint32_t before = 0;
 #pragma unroll
             for (int i = 0; i < kWave; ++i)

@@ -239,6 +239,27 @@ def test_causal_e4m3(q3k, hip, B, S, Hq, Hkv, cached, lengths):
              cached, lengths)
 
 
+# Lengths that the blocks' order has to cope with: below 0 and above the cache's, equal ones, the last of more than 64
+# sequences among themselves.
+LOWEST, HIGHEST = -2**31, 2**31 - 1
+ORDERS = {
+    "below": [-5, LOWEST, 40, -2, 17], "all-below": [LOWEST, -2, -3], "above": [HIGHEST, 64, 65, LOWEST, 64],
+    "equal": [33] * 6, "67": [(37 * i) % 65 for i in range(64)] + [12, LOWEST, 64],
+    "130": [64 - i % 65 for i in range(128)] + [-7, 3]}
+
+
+@pytest.mark.parametrize("form", ["causal", "tree", "tree-bf16"])
+@pytest.mark.parametrize("S", [1, 40])
+@pytest.mark.parametrize("order", sorted(ORDERS))
+def test_order_of_lengths(q3k, hip, order, S, form):
+    lengths = ORDERS[order]
+    B, trees = len(lengths), None
+    if form != "causal":
+        lengths = [n if n <= 0 else max(n, S) for n in lengths]
+        trees = _random_trees(np.random.default_rng(S + B), B, S)
+    _compare(q3k, hip, f"order of lengths {order} S {S} {form}", form != "tree-bf16", B, S, 4, 2, 128, 66, 64, lengths, trees)
+
+
 @pytest.mark.parametrize("D", [1, 64, 80, 256])
 def test_causal_e4m3_other_widths(q3k, hip, D):
     _compare(q3k, hip, f"attention e4m3 D {D}", True, 2, 3, 4, 2, D, 40, 37, [37, 2], workspaces=(True,))
