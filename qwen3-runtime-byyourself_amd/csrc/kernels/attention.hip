@@ -344,7 +344,7 @@ namespace q3k
                 __syncthreads(); // every wave is done with the V tiles
                 merge_groups<CW, KW>(
                     k_a, k_b, v_a, v_b, cw, kw, li, lg, o, m, l,
-                    [&](int dt, const f32x16_t &part, float inv, float) __attribute__((always_inline)) {
+                    [&](int dt, int, const f32x16_t &part, float inv, float) __attribute__((always_inline)) {
                         if (col_ok)
                             store_dims(a, split, sp, row, dt, lg, part, inv);
                     },
@@ -481,7 +481,7 @@ namespace q3k
                 __syncthreads(); // every wave is done with its tiles
                 merge_groups<1, KW>(
                     k_a, k_b, v_a, v_b, 0, kw, li, lg, o, m, l,
-                    [&](int dt, const f32x16_t &part, float inv, float) __attribute__((always_inline)) {
+                    [&](int dt, int, const f32x16_t &part, float inv, float) __attribute__((always_inline)) {
                         if (col_ok)
                             store_dims(a, split, sp, row, dt, lg, part, inv);
                     },

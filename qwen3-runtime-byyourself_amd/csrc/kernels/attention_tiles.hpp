@@ -300,16 +300,17 @@ namespace q3k
     // The KW groups' partial results of a column meet in LDS, in the tile
     // buffers: dims 32 dt .. + 31 of all waves in buffer dt (4 KiB a wave, 16
     // bytes a lane, so lanes hit distinct banks).  Group kw then merges and
-    // stores 4 / KW of the four parts: store_dims(part, O^T, 1 / sum, sum), and
-    // one lane a column its reference max and sum: store_ml.
+    // stores 4 / KW of the four parts, with eight groups half of one:
+    // store_dims(part, first, O^T, 1 / sum, sum) for quarters first .. of the
+    // part's elements, and one lane a column its reference max and sum: store_ml.
     template <int CW, int KW, typename StoreDims, typename StoreMl>
     __device__ __forceinline__ void merge_groups(unsigned char *b0, unsigned char *b1, unsigned char *b2,
                                                  unsigned char *b3, int cw, int kw, int li, int lg,
                                                  const f32x16_t (&o)[kAttD / 32], float m, float l,
                                                  StoreDims store_dims, StoreMl store_ml)
     {
-        static_assert(kAttD / 32 == 4 && 4 % KW == 0, "parts");
-        constexpr int kParts = 4 / KW;
+        static_assert(kAttD / 32 == 4 && (4 % KW == 0 || KW == 8), "parts");
+        constexpr int kParts = KW == 8 ? 1 : 4 / KW, kQuarters = KW == 8 ? 2 : 4;
         const int lane = 32 * lg + li, wave = kw * CW + cw;
         __shared__ float2 ml[KW][32 * CW];
         unsigned char *const bufs[4] = {b0, b1, b2, b3};
@@ -342,7 +343,7 @@ namespace q3k
 #pragma unroll
         for (int y = 0; y < kParts; ++y)
         {
-            const int dt = kw * kParts + y;
+            const int dt = KW == 8 ? kw / 2 : kw * kParts + y, first = KW == 8 ? 2 * (kw % 2) : 0;
             const unsigned char *buf = dt == 0 ? b0 : dt == 1 ? b1 : dt == 2 ? b2 : b3;
             f32x16_t r = f32x16_t{};
 #pragma unroll
@@ -350,16 +351,16 @@ namespace q3k
             {
                 const float4 *src = reinterpret_cast<const float4 *>(buf) + (x * CW + cw) * 4 * kWave;
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4)
+                for (int q4 = 0; q4 < kQuarters; ++q4)
                 {
-                    const float4 e = src[q4 * kWave + lane];
+                    const float4 e = src[(first + q4) * kWave + lane];
                     r[4 * q4] = __builtin_fmaf(w[x], e.x, r[4 * q4]);
                     r[4 * q4 + 1] = __builtin_fmaf(w[x], e.y, r[4 * q4 + 1]);
                     r[4 * q4 + 2] = __builtin_fmaf(w[x], e.z, r[4 * q4 + 2]);
                     r[4 * q4 + 3] = __builtin_fmaf(w[x], e.w, r[4 * q4 + 3]);
                 }
             }
-            store_dims(dt, r, inv, lsum);
+            store_dims(dt, first, r, inv, lsum);
         }
         if (lg == 0 && kw == 0)
             store_ml(mx, lsum);

@@ -59,7 +59,7 @@ namespace q3k
             float scale;
             int64_t rows;
             int32_t B;
-            bool ordered; // blocks take the sequences longest first
+            bool ordered; // decode blocks take the sequences longest first
             // the fast kernels: query blocks of a pair, slices of split_keys rows, their
             // results (unnormalised O^T [splits, rows, D], reference max and sum
             // [splits, rows, 2])
@@ -89,25 +89,14 @@ namespace q3k
             return bad ? 0 : static_cast<int32_t>(n);
         }
 
-        // Sequences of different lengths: blocks take them longest first, so that what
-        // starts last is short; and while all blocks are on the GPU at once, 256 to a round,
-        // every second round goes the other way, so that a CU's blocks are a long and a
-        // short one.  (64 sequences of 1024 to 4096 rows, 8 KV heads, in 512 blocks of two
-        // waves: X us, Y in the order given.)  Of more than 64 sequences each 64 are ordered
-        // among themselves.
-
-        // The unit that block i of `units` takes, units ordered longest first.
-        __device__ __forceinline__ int32_t long_and_short(int32_t i, int32_t units, int32_t resident)
-        {
-            constexpr int32_t kCus = 256;
-            const int32_t round = i / kCus;
-            if (units > resident || round % 2 == 0)
-                return i;
-            const int32_t last = units < (round + 1) * kCus ? units - 1 : (round + 1) * kCus - 1;
-            return last - (i - round * kCus);
-        }
-
-        // The sequence that comes `rank`-th by length; the whole wave calls it.
+        // The sequence that comes `rank`-th by length, or with a.ordered false in the order
+        // given; the whole wave calls it.  Decode blocks take sequences of different lengths
+        // longest first, so that what starts last is short (64 of 1024 to 4096 rows, 8 KV
+        // heads: 66.4 us, 78.0 in a random order; of 4000 to 16000 rows 231 us and 278; their
+        // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  In the block kernels,
+        // two blocks to a CU, it gave nothing (16 trees of 64 nodes, 40 heads: 124 to 130 us,
+        // 122 in a random order).  Of more than 64 sequences each 64 are ordered among
+        // themselves.
         __device__ __forceinline__ int32_t sequence_at(const CacheArgs &a, int32_t rank, int lane)
         {
             if (!a.ordered)
@@ -482,21 +471,23 @@ namespace q3k
                 qf[c] = as_bf8(qrow[CODES ? 4 * (c / 2) + 2 * lg + c % 2 : 2 * c + lg]);
         }
 
-        // Dims 32 dt .. + 31 of a query's result: bf16 O / l, or with slices the
-        // unnormalised O^T of this one.
-        __device__ __forceinline__ void store_dims(const CacheArgs &a, bool split, int sp, int64_t row, int dt, int lg,
+        // Dims 32 dt .. + 31 of a query's result, quarters first .. first + QUARTERS - 1 of
+        // them (O^T elements 0 .. of o): bf16 O / l, or with slices the unnormalised O^T of
+        // this one.
+        template <int QUARTERS>
+        __device__ __forceinline__ void store_dims(const CacheArgs &a, bool split, int sp, int64_t row, int dt, int first, int lg,
                                                    const f32x16_t &o, float inv, float l, Query q)
         {
             if (split)
             {
                 float *po = a.part_o + (static_cast<int64_t>(sp) * a.rows + row) * kAttD;
 #pragma unroll
-                for (int q4 = 0; q4 < 4; ++q4)
+                for (int q4 = 0; q4 < QUARTERS; ++q4)
                 {
                     float4 w = {o[4 * q4], o[4 * q4 + 1], o[4 * q4 + 2], o[4 * q4 + 3]};
                     if (q != Query::Sees)
                         w = {0.0f, 0.0f, 0.0f, 0.0f};
-                    *reinterpret_cast<float4 *>(po + dt * 32 + 8 * q4 + 4 * lg) = w;
+                    *reinterpret_cast<float4 *>(po + dt * 32 + 8 * (first + q4) + 4 * lg) = w;
                 }
                 return;
             }
@@ -504,14 +495,14 @@ namespace q3k
             const uint32_t fill = q == Query::Bad ? 0x7fc07fc0u : 0u;
             uint16_t *orow = a.out + row * kAttD;
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4)
+            for (int q4 = 0; q4 < QUARTERS; ++q4)
             {
                 uint2 w;
                 w.x = pack_rne(o[4 * q4] * inv, o[4 * q4 + 1] * inv);
                 w.y = pack_rne(o[4 * q4 + 2] * inv, o[4 * q4 + 3] * inv);
                 if (none)
                     w.x = w.y = fill;
-                *reinterpret_cast<uint2 *>(orow + dt * 32 + 8 * q4 + 4 * lg) = w;
+                *reinterpret_cast<uint2 *>(orow + dt * 32 + 8 * (first + q4) + 4 * lg) = w;
             }
         }
         // The slice's reference max and sum: those of a query without a row leave it
@@ -551,7 +542,10 @@ namespace q3k
         // a SIMD (64 KiB of LDS a block, at most 256 registers) and one's conversions and
         // softmax run beside the other's: with 64-key tiles and one wave a SIMD 64 ragged
         // sequences of up to 4096 rows took 73.3 us against 69.2, their trees of 5 nodes 51.3
-        // against 39.2.
+        // against 39.2.  The two are waves of one block (KW 8) where there is one to a CU or
+        // the keys are long (8 sequences of 1000 rows whole: 12.9 us, 15.8 with KW 4; 32
+        // ragged ones of up to 2500 29.7 and 38.4), else of two (64 of up to 1000: 23.3 us,
+        // 28.0 with KW 8).
         template <int KW, bool E4M3, bool TREE>
         __global__ __launch_bounds__(KW *kWave, E4M3 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
         {
@@ -570,8 +564,7 @@ namespace q3k
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
             // slices of a pair side by side
-            const int32_t unit = long_and_short(static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), 1024 / KW);
-            const int32_t sp = unit % a.splits, pair = unit / a.splits;
+            const int32_t sp = static_cast<int32_t>(blockIdx.x) % a.splits, pair = static_cast<int32_t>(blockIdx.x) / a.splits;
             const int32_t kvh = pair % a.Hkv;
             const int64_t b = sequence_at(a, pair / a.Hkv, lane);
             const int32_t S = static_cast<int32_t>(a.S);
@@ -749,9 +742,9 @@ namespace q3k
                     step(j + 1, k_b, v_b, s_b);
             }
             const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
-            const auto put_dims = [&](int dt, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+            const auto put_dims = [&](int dt, int first, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
                 if (col_ok)
-                    store_dims(a, split, sp, row, dt, lg, part, inv, sum, query);
+                    store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };
             const auto put_ml = [&](float mx, float sum) __attribute__((always_inline)) {
                 if (split && col_ok)
@@ -761,7 +754,7 @@ namespace q3k
             {
 #pragma unroll
                 for (int dt = 0; dt < kAttD / 32; ++dt)
-                    put_dims(dt, o[dt], 1.0f / l, l);
+                    put_dims(dt, 0, o[dt], 1.0f / l, l);
                 if (lg == 0)
                     put_ml(m, l);
             }
@@ -813,13 +806,14 @@ namespace q3k
             const int li = lane % 32, lg = lane / 32;
             // KV heads run fastest, so that with a multiple of 8 of them the blocks of a pair
             // meet on one XCD, whose L2 holds its K and V.  A tree's query blocks are equally
-            // long: sequences outermost, longest first; but a last block of fewer columns is
-            // lighter, and those come after all others.  Causal ones differ: slices
+            // long: sequences outermost; but a last block of fewer columns is lighter, and
+            // those come after all others.  Causal ones differ: slices
             // outermost, then the query blocks, longest first, then the sequences.
-            int32_t sp, qb, kvh, rank;
+            int32_t sp, qb, kvh;
+            int64_t b;
             if constexpr (TREE)
             {
-                int32_t unit = long_and_short(static_cast<int32_t>(blockIdx.x), static_cast<int32_t>(gridDim.x), KW == 1 ? 512 : 256);
+                int32_t unit = static_cast<int32_t>(blockIdx.x);
                 kvh = unit % a.Hkv;
                 unit /= a.Hkv;
                 const int32_t whole = static_cast<int32_t>(a.S) * g / kBlockCols; // query blocks of all their columns
@@ -827,7 +821,7 @@ namespace q3k
                 qb = light >= 0 ? whole : unit % whole;
                 unit = light >= 0 ? light : unit / whole;
                 sp = unit % a.splits;
-                rank = unit / a.splits;
+                b = unit / a.splits;
             }
             else
             {
@@ -836,9 +830,8 @@ namespace q3k
                 sp = rest / a.qblocks;
                 qb = a.qblocks - 1 - rest % a.qblocks;
                 kvh = pair % a.Hkv;
-                rank = pair / a.Hkv;
+                b = pair / a.Hkv;
             }
-            const int64_t b = sequence_at(a, rank, lane);
             const int32_t S = static_cast<int32_t>(a.S);
             const int32_t n_cols = S * g;
             const int32_t block_col = qb * kBlockCols;
@@ -1094,9 +1087,9 @@ namespace q3k
             if constexpr (TREE)
                 query = static_cast<Query>(tree.state[s_row - s_first]);
             const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
-            const auto put_dims = [&](int dt, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+            const auto put_dims = [&](int dt, int first, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
                 if (col_ok)
-                    store_dims(a, split, sp, row, dt, lg, part, inv, sum, query);
+                    store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };
             const auto put_ml = [&](float mx, float sum) __attribute__((always_inline)) {
                 if (split && col_ok)
@@ -1106,7 +1099,7 @@ namespace q3k
             {
 #pragma unroll
                 for (int dt = 0; dt < kAttD / 32; ++dt)
-                    put_dims(dt, o[dt], 1.0f / l, l);
+                    put_dims(dt, 0, o[dt], 1.0f / l, l);
                 if (lg == 0)
                     put_ml(m, l);
             }
@@ -1293,8 +1286,13 @@ namespace q3k
         int launch_fast(const char *what, const CacheArgs &a, int64_t B, const CacheAttnPlan &p, hipStream_t stream)
         {
             if (p.decode_waves > 0)
+            {
+                if constexpr (E4M3)
+                    if (p.decode_waves == 8)
+                        return launch_decode<8, E4M3, TREE>(what, a, B, stream);
                 return p.decode_waves == 1 ? launch_decode<1, E4M3, TREE>(what, a, B, stream)
                                            : launch_decode<4, E4M3, TREE>(what, a, B, stream);
+            }
             return p.key_groups == 1 ? launch_block<4, 1, 2, E4M3, TREE>(what, a, B, stream)
                                      : launch_block<2, 4, 1, E4M3, TREE>(what, a, B, stream);
         }
@@ -1387,7 +1385,7 @@ namespace q3k
                 if (p.bytes > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < p.bytes))
                     p = plan_cache_attention(B, a.S, a.Hq, a.Hkv, a.cached, e4m3, tree, ragged, false);
                 a.B = static_cast<int32_t>(B);
-                a.ordered = ragged && B > 1 && (p.splits == 1 || p.decode_waves == 0);
+                a.ordered = ragged && B > 1 && p.splits == 1 && p.decode_waves > 0;
                 a.splits = p.splits;
                 a.split_keys = p.split_keys;
                 a.part_o = static_cast<float *>(workspace);

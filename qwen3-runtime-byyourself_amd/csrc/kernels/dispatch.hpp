@@ -431,7 +431,7 @@ namespace q3k
 
     struct CacheAttnPlan
     {
-        int32_t decode_waves = 0; // waves of a decode block (1 or 4); 0: the block kernel
+        int32_t decode_waves = 0; // waves of a decode block (1, 4 or, e4m3, 8); 0: the block kernel
         int32_t key_groups = 1;   // block kernel: groups of waves that divide the keys (1 or 4)
         int32_t splits = 1;       // slices of split_keys rows
         int32_t split_keys = INT32_MAX;
@@ -442,38 +442,51 @@ namespace q3k
     constexpr int64_t kCacheMaxBlocks = 2048;
     constexpr int32_t kCacheDecodeTile = 32; // rows of a decode wave's tile
     constexpr int32_t kCacheBlockTile = 128; // slices of the block kernels are whole tiles of both
-    // What a call expects of sequences whose lengths the host does not know, as a share of
-    // the longest: of the decode kernel's time, and of the block kernels'.
-    constexpr double kRaggedDecode = 0.85, kRaggedBlock = 0.9;
+    // What a call expects of sequences whose lengths the host does not know: this share of
+    // the longest, in the decode kernel and in the block kernels.
+    constexpr double kRaggedDecode = 0.87, kRaggedBlock = 0.8;
 
     inline constexpr double cache_row_bytes(bool e4m3) { return e4m3 ? 2.0 * (kAttHeadDim + 1) : 4.0 * kAttHeadDim; }
 
-    // Estimated time in us of the decode kernel in blocks of four waves and slices of
-    // split_keys rows (>= cached: whole).  A wave takes 1.7 us a tile of codes and 1.4 us a
-    // tile of bf16 rows on a busy chip, with two blocks on a CU (e4m3) 1.85 times that; all
-    // CUs read 5.1 TB/s together and one 31 GB/s; start and end take 2.7 us, another round
-    // of blocks 1.9 us, the merge 3.2 us and its bytes.  Constants fitted to 357 shapes of 1
-    // to 64 sequences, 150 to 32000 rows, 1 to 32 columns, cut into 1 to 64 slices: the
-    // slices taken so are 1.0% slower than the best of each on average, 18% at worst.
-    inline double cache_decode_us(int64_t pairs, int64_t cols, int64_t cached, bool e4m3, bool ragged, int64_t split_keys)
+    // Estimated time in us of the decode kernel in blocks of `waves` waves and slices of
+    // split_keys rows (>= cached: whole).  A wave takes 1.45 us a tile of codes with four
+    // waves on its CU and 1.8 times that with eight, 1.85 times in two blocks, and 1.4 us a
+    // tile of bf16 rows; a CU reads 34 GB/s of them; start and end take 3.2 us, 0.5 more with
+    // eight waves, another round of blocks 3.5 us, the merge 3 us and its bytes.  Whole
+    // sequences of different lengths, longest first, take the longest one's time or the
+    // CUs' share of all, and another round of eight waves twice as much.  Fitted
+    // to 238 shapes over e4m3 and 119 over bf16 of 1 to 64 sequences, 150 to 32000 rows, 1 to
+    // 32 columns, cut into 1 to 64 slices: the form taken so is 1.0% and 0.7% slower than the
+    // best of each on average, 16% at worst; over 146 of 12 to 300 sequences of different
+    // lengths 1.7% and 26%.
+    inline double cache_decode_us(int64_t pairs, int64_t cols, int64_t cached, bool e4m3, bool ragged, int waves, int64_t split_keys)
     {
         const double share = ragged ? kRaggedDecode : 1.0;
         const int64_t keys = split_keys < cached ? split_keys : cached, slices = blocks_for(cached, keys);
-        const double blocks = static_cast<double>(pairs * slices), slots = e4m3 ? 512.0 : 256.0;
+        const double blocks = static_cast<double>(pairs * slices), slots = e4m3 && waves == 4 ? 512.0 : 256.0;
         const double live = ragged && slices > 1 ? blocks * share : blocks;
-        const double step = (e4m3 ? 1.7 : 1.4) * (e4m3 && live > 256.0 ? 1.85 : 1.0);
-        double rounds = live / slots;
-        rounds = rounds <= 1.0 ? 1.0 : rounds < 2.5 ? static_cast<double>(static_cast<int64_t>(rounds + 0.999999)) : rounds + 0.5;
-        double us = step * static_cast<double>(blocks_for(blocks_for(keys, kCacheDecodeTile), 4)) * rounds;
-        if (ragged && slices == 1 && rounds > 1.0)
-            us *= 0.5 * (1.0 + share);
+        const double alone = e4m3 ? (waves == 8 ? 1.8 : 1.0) * 1.45 : 1.4;
+        const double step = e4m3 && waves == 4 && live > 256.0 ? 1.85 * alone : alone;
+        const double tiles = static_cast<double>(blocks_for(blocks_for(keys, kCacheDecodeTile), waves));
+        double rounds = live / slots, us = 0.0;
+        if (ragged && slices == 1)
+        {
+            const double queued = (waves == 8 ? 0.72 : 0.8) * rounds * step;
+            us = tiles * (queued > alone ? queued : alone);
+            rounds = rounds > 1.0 ? waves == 8 ? 2.0 * rounds - 1.0 : rounds : 1.0;
+        }
+        else
+        {
+            rounds = rounds <= 1.0 ? 1.0 : rounds < 2.5 ? static_cast<double>(static_cast<int64_t>(rounds + 0.999999)) : rounds + 0.5;
+            us = tiles * rounds * step;
+        }
         const double bytes = static_cast<double>(pairs) * static_cast<double>(cached) * share * cache_row_bytes(e4m3);
         const double busy = live < 256.0 ? live : 256.0;
-        us = us > bytes / 5.1e6 ? us : bytes / 5.1e6;
-        us = us > bytes / (busy * 31.0e3) ? us : bytes / (busy * 31.0e3);
-        us += 2.7 + 1.9 * (rounds - 1.0);
+        us = us > bytes / 8.0e6 ? us : bytes / 8.0e6;
+        us = us > bytes / (busy * 34.0e3) ? us : bytes / (busy * 34.0e3);
+        us += 3.2 + (waves == 8 ? 0.5 : 0.0) + 3.5 * (rounds - 1.0);
         if (slices > 1)
-            us += 3.2 + 0.01 * static_cast<double>(slices) + live * static_cast<double>(cols) * (2.0 * (kAttHeadDim + 2) * 4) / 3.0e6;
+            us += 3.0 + 0.01 * static_cast<double>(slices) + live * static_cast<double>(cols) * ((kAttHeadDim + 2) * 4) / 1.6e6;
         return us;
     }
 
@@ -482,23 +495,29 @@ namespace q3k
     {
         const int64_t pairs = B * Hkv, cols = S * (Hq / Hkv);
         CacheAttnPlan p;
-        p.decode_waves = cached <= kCacheDecodeTile ? 1 : 4; // one tile: nothing to divide
-        if (!can_split)
+        p.decode_waves = 1;
+        if (cached <= kCacheDecodeTile) // one tile: nothing to divide
             return p;
-        double best = cache_decode_us(pairs, cols, cached, e4m3, ragged, cached);
-        for (const int slices : {2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64})
+        double best = -1.0;
+        for (const int waves : {4, 8})
         {
-            if (slices > kAttMaxSplits || slices > kCacheMaxBlocks / pairs)
-                break;
-            const int64_t keys = blocks_for(blocks_for(cached, slices), kCacheDecodeTile) * kCacheDecodeTile;
-            if (keys >= cached || keys < 2 * kCacheDecodeTile)
+            if (waves == 8 && !e4m3) // its tiles fill the LDS with four
                 continue;
-            const double us = cache_decode_us(pairs, cols, cached, e4m3, ragged, keys);
-            if (us >= best)
-                continue;
-            best = us;
-            p.split_keys = static_cast<int32_t>(keys);
-            p.splits = static_cast<int32_t>(blocks_for(cached, keys));
+            for (const int slices : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64})
+            {
+                if (slices > 1 && (!can_split || slices > kAttMaxSplits || slices > kCacheMaxBlocks / pairs))
+                    break;
+                const int64_t keys = blocks_for(blocks_for(cached, slices), kCacheDecodeTile) * kCacheDecodeTile;
+                if (slices > 1 && (keys >= cached || keys < 2 * kCacheDecodeTile))
+                    continue;
+                const double us = cache_decode_us(pairs, cols, cached, e4m3, ragged, waves, slices > 1 ? keys : cached);
+                if (best >= 0.0 && us >= best)
+                    continue;
+                best = us;
+                p.decode_waves = waves;
+                p.splits = slices > 1 ? static_cast<int32_t>(blocks_for(cached, keys)) : 1;
+                p.split_keys = slices > 1 ? static_cast<int32_t>(keys) : INT32_MAX;
+            }
         }
         if (p.splits > 1)
             p.bytes = p.splits * B * S * Hq * (kAttHeadDim + 2) * 4;
@@ -506,41 +525,47 @@ namespace q3k
     }
 
     // Estimated time in us of the block kernels, 128 columns and one key group or 64 columns
-    // and four.  A 64-key tile takes a block alone on its CU 1.85 us (0.84 with four groups)
-    // and 1.0 us (1.25) of CU time where blocks queue or share a CU; a query block that is
-    // not full costs 0.35 of a full one and its columns' part of the rest; start and end 5.2
-    // us (4.2).  Causal query blocks see between cached - S and cached rows.  Fitted to 400
-    // shapes of 1 to 64 sequences and 12 to 400 queries or nodes: 1.1% slower than the best
-    // of the one to twenty forms of each on average, 36% at worst (4 trees of 130 nodes).
+    // and four.  A 64-key tile takes a block alone on its CU 1.7 us (0.93 with four groups)
+    // and 0.81 us (1.54) of CU time where blocks queue or share a CU; a query block that is
+    // not full costs 0.64 of a full one and its columns' part of the rest; start and end 9.8
+    // us (4.7).  Causal query blocks see between cached - S and cached rows.  Fitted to 550
+    // shapes of 1 to 100 sequences and 12 to 400 queries or nodes: 0.8% slower than the best
+    // of the one to twenty forms of each on average, 28% at worst.
     inline double cache_block_us(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool tree, bool ragged,
                                  int key_groups, int64_t split_keys)
     {
         const int32_t G = Hq / Hkv, block_cols = attn_block_cols(key_groups);
         const int64_t pairs = B * Hkv, cols = S * G, qblocks = blocks_for(cols, block_cols);
         const double share = ragged ? kRaggedBlock : 1.0, rows = static_cast<double>(cached);
-        const double alone = key_groups == 1 ? 1.85 : 0.84, busy = key_groups == 1 ? 1.0 : 1.25;
-        double mean = 1.0;
+        const double alone = key_groups == 1 ? 1.7 : 0.93, busy = key_groups == 1 ? 0.81 : 1.54;
+        double first = rows; // rows that the first query block sees
         if (!tree)
         {
             const int64_t positions = blocks_for(block_cols, G) < S ? blocks_for(block_cols, G) : S;
-            mean = 0.5 * (static_cast<double>(cached - S + positions) + rows) / rows;
+            first = static_cast<double>(cached - S + positions);
         }
+        const double mean = 0.5 * (first + rows) / rows;
         const int64_t keys = split_keys < cached ? split_keys : cached, slices = blocks_for(cached, keys);
         const double longest = alone * static_cast<double>(blocks_for(keys, 64));
         double weight = static_cast<double>(cols / block_cols);
         if (cols % block_cols != 0)
-            weight += 0.35 + 0.65 * static_cast<double>(cols % block_cols) / block_cols;
+            weight += 0.64 + 0.36 * static_cast<double>(cols % block_cols) / block_cols;
         const double per_cu = static_cast<double>(pairs) * weight * rows * share * mean / 64.0 / 256.0;
         double blocks = static_cast<double>(pairs * qblocks);
         if (slices > 1)
         {
-            const double n = static_cast<double>(slices) * share * mean + (ragged || !tree ? 0.5 : 0.0);
+            // slices of a block, on average: of four blocks spread over the range
+            double n = 0.0;
+            for (int i = 0; i < 4; ++i)
+                n += 0.25 * static_cast<double>(blocks_for(static_cast<int64_t>(first + (rows - first) * i / 3.0), keys));
+            if (ragged)
+                n = n * share + 0.25;
             blocks *= n > 1.0 ? n : 1.0;
         }
         double us = longest;
         if (blocks > 256.0)
         {
-            double queued = per_cu * busy + 0.35 * longest;
+            double queued = per_cu * busy + 0.52 * longest;
             if (key_groups == 1 && blocks <= 512.0)
             {
                 const double both = (blocks / 256.0) * (longest / alone * busy) * (0.5 + 0.5 * share);
@@ -549,11 +574,11 @@ namespace q3k
             us = us > queued ? us : queued;
         }
         const double rounds = blocks / (key_groups == 1 ? 512.0 : 256.0);
-        us += (key_groups == 1 ? 5.2 : 4.2) * (rounds <= 1.0 ? 1.0 : rounds + 0.5);
+        us += (key_groups == 1 ? 9.8 : 4.7) * (rounds <= 1.0 ? 1.0 : rounds + 0.5);
         const double read = static_cast<double>(pairs) * rows * share * cache_row_bytes(e4m3) / 5.0e6;
         us = us > read ? us : read;
         if (slices > 1)
-            us += 3.0 + static_cast<double>(B * S * Hq * slices) * share * (2.0 * (kAttHeadDim + 2) * 4) / 5.6e6;
+            us += 4.7 + static_cast<double>(B * S * Hq * slices) * share * ((kAttHeadDim + 2) * 4) / 4.1e6;
         return us;
     }
 
