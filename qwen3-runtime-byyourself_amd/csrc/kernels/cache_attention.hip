@@ -14,11 +14,11 @@
 // head) columns to a wave.
 //   Few columns (at most 32 to a (sequence, KV head): decode, small trees): the
 //   block's waves divide the keys and stream their own tiles of 32 keys through
-//   LDS.  Codes stay 8 bits wide until a fragment is in registers: K's with ds_read_b128, 16 dims of a key, converted
-//   to two bf16 fragments with the key's scale (a lane holds one key, so the scale
-//   is one register); V's with the 8-bit transpose read, 8 keys of a dim, converted
-//   without a scale, which is multiplied into the weights instead (there a lane
-//   holds one column and 16 keys of each 32).
+//   LDS.  Codes stay 8 bits wide until a fragment is in registers: K's with
+//   ds_read_b128, 16 dims of a key, converted to two bf16 fragments with the key's
+//   scale (a lane holds one key, so the scale is one register); V's with the 8-bit
+//   transpose read, 8 keys of a dim, converted without a scale, which is multiplied
+//   into the weights instead (there a lane holds one column and 16 keys of each 32).
 //   More columns (larger trees, prefill): a block of waves shares its K and V tiles
 //   as bf16; codes are converted once, on their way into LDS.
 // The mask only touches the tiles at a sequence's end.  A masked score is -inf, so
@@ -29,7 +29,9 @@
 //
 // Generic path (any head_dim <= 256, any strides and alignment): one wave per
 // query row, its rows in order, lanes over the head dimension, the running
-// maximum and sum of the softmax in fp32.
+// maximum and sum of the softmax in fp32.  It is bound by the chain of one row after
+// another and reads K and V once for each query head: 50 to 500 times the time of the
+// others where both could run (64 ragged sequences of up to 4096 rows: 4674 us, 66).
 #include "attention_tiles.hpp"
 #include "dispatch.hpp"
 #include "kv_e4m3.hpp"
@@ -546,6 +548,9 @@ namespace q3k
         // the keys are long (8 sequences of 1000 rows whole: 12.9 us, 15.8 with KW 4; 32
         // ragged ones of up to 2500 29.7 and 38.4), else of two (64 of up to 1000: 23.3 us,
         // 28.0 with KW 8).
+        // 64 ragged sequences of 1024 to 4096 rows, 32 / 8 heads: 66 to 73 us, 339 MB at 4.7
+        // to 5.1 TB/s of the 5.4 to 5.9 that the access pattern reaches; one of 8191 rows,
+        // 16 / 8 heads, cut into slices, 11.4 us, of which the merge takes 2.8.
         template <int KW, bool E4M3, bool TREE>
         __global__ __launch_bounds__(KW *kWave, E4M3 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
         {
@@ -780,6 +785,13 @@ namespace q3k
         //   converted into them: two barriers a tile, half the LDS for tiles and no
         //   registers for loads in flight (holding the codes in registers instead spilled
         //   or cost the second block of a CU).
+        // What bounds it is the softmax beside the matrix instructions, as in the bf16
+        // attention.  512 queries over 8192 rows, 32 / 8 heads, e4m3, in 4 slices: 95 us and 8
+        // for the merge, 643 TFLOP/s of the products, matrix cores busy 44%.  16 ragged trees
+        // of 64 nodes over up to 4160 bf16 rows, 40 / 8 heads: 117 to 123 us, 440 to 455
+        // TFLOP/s, 384 blocks of unequal length, two to a CU.  Four groups with 64 columns
+        // are for few blocks (4 trees of 64 nodes over 2000 rows: 38.4 us, 40.7 with 128
+        // columns) and lose where there are many (64 of 16 nodes over 1000: 49.2 and 43.2).
         template <int CW, int KW, int HH, bool E4M3, bool TREE>
         __global__ __launch_bounds__(CW *KW *kWave, 2) void cache_block_kernel(CacheArgs a)
         {
@@ -1136,7 +1148,8 @@ namespace q3k
             return block <= a.split_keys ? 0 : own <= 0 ? 1 : (own - 1) / a.split_keys + 1;
         }
 
-        // Few rows, many slices: a block of four waves a row.  Lane i of each wave reads
+        // Few rows, many slices: a block of four waves a row (32 rows of 32 slices 2.8 us,
+        // 832 of 16 3.9).  Lane i of each wave reads
         // slice i's reference max and sum, wave w the unnormalised O^T of slices w, w + 4,
         // ..., all before any is used; weights 2^(m_i - max m), then sum w O / sum w l.
         constexpr int kMergeWaves = 4;
@@ -1196,7 +1209,8 @@ namespace q3k
         }
 
         // Many rows: 16 lanes a row, 8 dims a lane, four slices at a time; every lane works
-        // the weights out for itself, so nothing is exchanged.
+        // the weights out for itself, so nothing is exchanged.  Memory bounds it: 16384 rows
+        // of 4 slices 7.7 us, 38 MB at 5.0 TB/s.
         constexpr int kMergeSlices = 4;
         constexpr int kMergeRows = kBlock / 16;
 
@@ -1302,8 +1316,9 @@ namespace q3k
         bool fast(const CacheArgs &a, bool e4m3)
         {
             // (tile ends are counted in 32 bits)
-            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || a.cached > INT32_MAX - 4 * kAttKeyTile || !aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) ||
-                !aligned_to(a.out, 8))
+            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || a.cached > INT32_MAX - 4 * kAttKeyTile)
+                return false;
+            if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned_to(a.out, 8))
                 return false;
             if (e4m3)
                 return aligned_to(a.scales, 2);

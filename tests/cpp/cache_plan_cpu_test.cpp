@@ -15,7 +15,7 @@ namespace
     {
         using namespace q3k;
         const int32_t heads[][2] = {{16, 8}, {32, 8}, {40, 8}, {64, 8}, {2, 1}, {4, 1}, {5, 1}, {8, 1}, {32, 1}};
-        int64_t cut = 0, whole = 0;
+        int64_t cut = 0, whole = 0, waves[9] = {};
         for (const auto &h : heads)
             for (const int64_t B : {1, 2, 5, 16, 40, 64, 200, 3000})
                 for (const int64_t S : {1, 2, 7, 33, 100, 256, 1000})
@@ -35,6 +35,10 @@ namespace
                             const CacheAttnPlan p = plan_cache_attention(B, S, h[0], h[1], cached, e4m3, tree, ragged, true);
                             const bool decode = S * (h[0] / h[1]) <= kAttColsPerWave;
                             require((p.decode_waves > 0) == decode, what + ": kernel");
+                            require(!decode || p.decode_waves == 1 || p.decode_waves == 4 || (e4m3 && p.decode_waves == 8),
+                                    what + ": a block of waves that is not built");
+                            require(decode || p.key_groups == 1 || p.key_groups == 4, what + ": key groups that are not built");
+                            waves[decode ? p.decode_waves : 0] += 1;
                             require((p.splits > 1) == (p.bytes > 0), what + ": a size without slices, or slices without");
                             require(p.bytes <= bytes, what + ": the slices need more than the workspace");
                             require(p.bytes == 0 || p.bytes == p.splits * B * S * h[0] * (kAttHeadDim + 2) * 4, what + ": size");
@@ -54,6 +58,7 @@ namespace
                     }
                 }
         require(cut > 10000 && whole > 10000, "the shapes cover whole and cut keys");
+        require(waves[1] > 0 && waves[4] > 0 && waves[8] > 0 && waves[0] > 0, "the shapes cover every kernel");
     }
 } // namespace
 
