@@ -237,41 +237,88 @@ namespace q3k
 
         // ---- masks -----------------------------------------------------------------
 
-        // The masks of a block's positions in a tree: word w + 1 of a position holds
-        // the bits of nodes 32 w .. + 31 that it sees, word 0 stands for the context
-        // before them and the last word for what lies behind.
-        template <bool TREE, int POSITIONS, int NODES>
+        // Nodes base .. base + 63 of a tree of T, one a lane of a wave, with `up` its parent:
+        // which of them are the node's ancestors or itself, and where the way up leaves them
+        // (an earlier node, or -1, -2, or kBadParent for a parent that cannot be).  Each step
+        // joins a node's stretch of the way with that of the node where it ends, so 64 nodes
+        // take at most six (a chain of 128 nodes in two waves: 22 us a call of 4 trees, 37
+        // when each position went up node by node).
+        constexpr int32_t kBadParent = -3;
+
+        template <typename Mask>
+        __device__ __forceinline__ void ancestors(int32_t up, int32_t base, int32_t T, int lane, Mask &mask, int32_t &end)
+        {
+            const int32_t node = base + lane;
+            mask = Mask{1} << (lane % (8 * static_cast<int>(sizeof(Mask))));
+            end = node >= T ? -2 : up < -2 || up >= node ? kBadParent : up;
+            while (__ballot(end >= base) != 0)
+            {
+                const int src = end >= base ? end - base : lane;
+                Mask m;
+                if constexpr (sizeof(Mask) == 4)
+                    m = static_cast<uint32_t>(__shfl(static_cast<int>(mask), src, kWave));
+                else
+                    m = static_cast<uint32_t>(__shfl(static_cast<int>(mask), src, kWave)) |
+                        static_cast<uint64_t>(static_cast<uint32_t>(__shfl(static_cast<int>(mask >> 32), src, kWave))) << 32;
+                const int32_t e = __shfl(end, src, kWave);
+                if (end >= base)
+                {
+                    mask |= m;
+                    end = e;
+                }
+            }
+        }
+        __device__ __forceinline__ Query query_of(int32_t end)
+        {
+            return end == -1 ? Query::Sees : end == -2 ? Query::Empty : Query::Bad;
+        }
+
+        // The masks of a tree's nodes: word w + 1 of a node holds the bits of nodes 32 w ..
+        // + 31 that it sees, word 0 stands for the context before them and the last word for
+        // what lies behind.
+        template <bool TREE>
         struct TreeMasks
         {
-            static constexpr int kWords = NODES / 32 + 2;
-            int32_t parent[NODES];
-            uint32_t mask[POSITIONS][kWords];
-            int32_t state[POSITIONS];
+            static constexpr int kWords = kTreeMaxNodes / 32 + 2;
+            uint32_t mask[kTreeMaxNodes][kWords];
+            int32_t end[kTreeMaxNodes]; // -1, -2 or kBadParent
         };
-        template <int POSITIONS, int NODES>
-        struct TreeMasks<false, POSITIONS, NODES>
+        template <>
+        struct TreeMasks<false>
         {
         };
 
-        // Positions first .. first + count - 1 of a tree of T nodes; every thread of the
-        // block calls it.
-        template <int POSITIONS, int NODES>
-        __device__ __forceinline__ void tree_masks(TreeMasks<true, POSITIONS, NODES> &t, const int32_t *parents, int T, int first,
-                                                   int count, int thread, int threads)
+        // Every wave of the block calls it, `up` the parent of node 64 wave + lane: 64 nodes
+        // at a time, which look up the way above them in the nodes before.
+        __device__ __forceinline__ void tree_masks(TreeMasks<true> &t, int32_t up, int32_t T, int wave, int lane)
         {
-            for (int i = thread; i < T; i += threads)
-                t.parent[i] = parents[i];
-            constexpr int W = TreeMasks<true, POSITIONS, NODES>::kWords;
-            for (int i = thread; i < count * W; i += threads)
-                t.mask[i / W][i % W] = i % W == 0 ? 0xffffffffu : 0u;
-            __syncthreads();
-            for (int i = thread; i < count; i += threads)
+            constexpr int kWords = TreeMasks<true>::kWords;
+            const int32_t base = kWave * wave, node = base + lane;
+            uint64_t mask = 0;
+            int32_t end = -2;
+            if (base < T)
+                ancestors(up, base, T, lane, mask, end);
+            for (int32_t done = 0; done < T; done += kWave)
             {
-                uint32_t *row = t.mask[i];
-                t.state[i] = static_cast<int32_t>(
-                    walk_up(t.parent, first + i, [&](int32_t u) { row[1 + u / 32] |= 1u << (u % 32); }));
+                if (done == base)
+                {
+                    const int32_t above = end;
+                    if (above >= 0)
+                        end = t.end[above];
+                    t.end[node] = end;
+                    t.mask[node][0] = 0xffffffffu;
+                    t.mask[node][kWords - 1] = 0;
+#pragma unroll
+                    for (int w = 0; w < kWords - 2; ++w)
+                    {
+                        uint32_t bits = above >= 0 ? t.mask[above][1 + w] : 0u;
+                        if (w / 2 == wave)
+                            bits = static_cast<uint32_t>(mask >> (32 * (w % 2)));
+                        t.mask[node][1 + w] = bits;
+                    }
+                }
+                __syncthreads();
             }
-            __syncthreads();
         }
 
         // Which of the 32 keys from `off` nodes into the tree (below 0: the context) a
@@ -283,6 +330,13 @@ namespace q3k
             i = i < 0 ? 0 : i < W ? i : W - 1;
             j = j < 0 ? 0 : j < W ? j : W - 1;
             return __builtin_amdgcn_alignbit(row[j], row[i], static_cast<uint32_t>(off) & 31u);
+        }
+        // The same for a tree of up to 32 nodes, `mask` those that the position sees.
+        __device__ __forceinline__ uint32_t tree_window(uint32_t mask, int32_t off)
+        {
+            return off >= 0 ? (off < 32 ? mask >> off : 0u)
+                            : off > -32 ? __builtin_amdgcn_alignbit(mask, 0xffffffffu, static_cast<uint32_t>(off) & 31u)
+                                        : 0xffffffffu;
         }
 
         // Which of the 32 keys from key0 are at most `last`.
@@ -564,7 +618,6 @@ namespace q3k
             __shared__ uint32_t s_a[E4M3 ? KW * kWave : 1];
             __shared__ uint32_t s_b[E4M3 ? KW * kWave : 1];
             __shared__ __attribute__((aligned(16))) float v_scale[E4M3 ? KW * kWave : 4];
-            __shared__ TreeMasks<TREE, kAttColsPerWave, kAttColsPerWave> tree;
             const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
@@ -593,16 +646,14 @@ namespace q3k
             const int32_t context = n_keys - S;                       // rows before the queries' own
             const int32_t all_seen = TREE ? context : context + 1;    // rows every query sees
 
+            int32_t parent = 0;
             if constexpr (TREE)
-                tree_masks(tree, a.parents + b * a.parents_stride, S, 0, S, threadIdx.x, KW * kWave);
+                parent = a.parents[b * a.parents_stride + (lane < S ? lane : S - 1)];
             // the lane's column; lanes past the last one repeat a row of the last position
             const int32_t s_col = li / g;
             const int h_col = kvh * g + li % g;
             const bool col_ok = s_col < S;
             const int32_t s_row = col_ok ? s_col : S - 1;
-            Query query = Query::Sees;
-            if constexpr (TREE)
-                query = static_cast<Query>(tree.state[s_row]);
 
             constexpr int64_t kElement = E4M3 ? 1 : 2;
             const unsigned char *kbase = static_cast<const unsigned char *>(a.k) + (b * a.ks0 + kvh * a.ks2) * kElement;
@@ -640,6 +691,18 @@ namespace q3k
             {
                 load_k(1, k_b, s_b);
                 load_v(1, v_b);
+            }
+            // each wave has the tree to itself, a node a lane
+            Query query = Query::Sees;
+            uint32_t tree = 0; // the nodes that the lane's column sees
+            if constexpr (TREE)
+            {
+                static_assert(kAttColsPerWave <= 32, "nodes of a word");
+                uint32_t mask;
+                int32_t end;
+                ancestors(parent, 0, S, lane, mask, end);
+                tree = static_cast<uint32_t>(__shfl(static_cast<int>(mask), s_row, kWave));
+                query = query_of(__shfl(end, s_row, kWave));
             }
             int v_off[kAttD / 32];
             if constexpr (E4M3)
@@ -683,7 +746,7 @@ namespace q3k
                 if (masked)
                 {
                     if constexpr (TREE)
-                        seen[0] = tree_window(tree.mask[s_row], key0 - context);
+                        seen[0] = tree_window(tree, key0 - context);
                     else
                         seen[0] = causal_window(key0, context + s_row);
                     mask_scores<1>(sacc, seen, lg);
@@ -810,7 +873,7 @@ namespace q3k
             __shared__ __attribute__((aligned(16))) unsigned char v_b[kSecond];
             __shared__ uint32_t k_scales[E4M3 ? kWaves * kWave : 1];
             __shared__ uint32_t v_scales[E4M3 ? kWaves * kWave : 1];
-            __shared__ TreeMasks<TREE, kBlockCols, kTreeMaxNodes> tree;
+            __shared__ TreeMasks<TREE> tree;
 
             const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
             const int cw = wave % CW, kw = wave / CW;
@@ -873,8 +936,13 @@ namespace q3k
             const int steps = (tile_end - tile0 + KW - 1) / KW;
             const int mine = first < tile_end ? (tile_end - first + KW - 1) / KW : 0;
 
+            int32_t parent = 0;
             if constexpr (TREE)
-                tree_masks(tree, a.parents + b * a.parents_stride, S, s_first, s_last - s_first + 1, threadIdx.x, kWaves * kWave);
+            {
+                static_assert(kWaves * kWave >= kTreeMaxNodes, "a thread a node");
+                const int32_t node = static_cast<int32_t>(threadIdx.x);
+                parent = a.parents[b * a.parents_stride + (node < S ? node : S - 1)];
+            }
             // this lane's column
             const int32_t wave_col = block_col + 32 * cw;
             const int32_t col = wave_col + li;
@@ -955,7 +1023,7 @@ namespace q3k
                 for (int hh = 0; hh < HH; ++hh)
                 {
                     if constexpr (TREE)
-                        seen[hh] = tree_window(tree.mask[s_row - s_first], key0 + 32 * hh - context);
+                        seen[hh] = tree_window(tree.mask[s_row], key0 + 32 * hh - context);
                     else
                         seen[hh] = causal_window(key0 + 32 * hh, context + s_row);
                 }
@@ -1006,6 +1074,10 @@ namespace q3k
                 // o holds the tiles before this one at the previous reference
                 rescale(o, alpha);
             };
+            auto masks = [&]() __attribute__((always_inline)) {
+                if constexpr (TREE)
+                    tree_masks(tree, parent, S, wave, lane);
+            };
             using no_pv = std::integral_constant<bool, false>;
             using with_pv = std::integral_constant<bool, true>;
             if constexpr (E4M3)
@@ -1035,6 +1107,7 @@ namespace q3k
                     stage(first, kbase, k_b, k_scales);
                     stage(first, vbase, v_b, v_scales);
                 }
+                masks();
                 wait_loads<0>();
                 if (mine > 0)
                     convert(k_b, k_scales, 0, k_a, kslot);
@@ -1071,6 +1144,7 @@ namespace q3k
                     load_k(first, k_a);
                     load_v(first, v_a);
                 }
+                masks();
                 wait_loads<0>();
                 __syncthreads();
                 // V of step j sits in v_a when j is even, else in v_b
@@ -1097,7 +1171,7 @@ namespace q3k
 
             Query query = Query::Sees;
             if constexpr (TREE)
-                query = static_cast<Query>(tree.state[s_row - s_first]);
+                query = query_of(tree.end[s_row]);
             const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
             const auto put_dims = [&](int dt, int first, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
                 if (col_ok)

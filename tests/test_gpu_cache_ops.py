@@ -293,6 +293,27 @@ def test_tree(q3k, hip, B, T, Hq, Hkv, cached, lengths, e4m3):
              cached, lengths, trees)
 
 
+def _long_ways(T):
+    """Chains, ways that jump far back, and wrong parents and padding whose descendants lie far behind them."""
+    chain = np.arange(-1, T - 1, dtype=np.int32)
+    broken, padded, jumps, below = chain.copy(), chain.copy(), chain.copy(), chain.copy()
+    broken[T // 3] = T - 1                       # a later node
+    padded[T // 2] = -2
+    jumps[T // 4:] = np.arange(T - T // 4) % (T // 4)
+    below[T // 5] = -3
+    below[T // 4:] = np.arange(T // 4, T) // 2
+    below[-1] = -2**31
+    return np.stack([chain, broken, padded, jumps, below])
+
+
+@pytest.mark.parametrize("e4m3", [False, True])
+@pytest.mark.parametrize("T,Hq,Hkv", [(7, 4, 1), (32, 2, 2), (33, 2, 1), (64, 2, 1), (65, 4, 2), (128, 2, 1), (200, 4, 1), (256, 2, 2)])
+def test_tree_long_ways(q3k, hip, T, Hq, Hkv, e4m3):
+    trees = _long_ways(T)
+    _compare(q3k, hip, f"tree long ways e4m3 {e4m3} T {T} heads {Hq}/{Hkv}", e4m3, 5, T, Hq, Hkv, 128, T + 40, T + 35,
+             [T + 35, T, T + 3, T + 34, T + 20], trees)
+
+
 @pytest.mark.parametrize("strides,D", [("head-major", 128), ("odd", 128), ("odd", 96), (None, 64)])
 def test_tree_strides(q3k, hip, strides, D):
     trees = _random_trees(np.random.default_rng(3), 2, 9)
