@@ -417,6 +417,10 @@ namespace q3k
             return make_uint2(static_cast<uint32_t>(c.x), static_cast<uint32_t>(c.y));
         }
 
+        // O^T += V^T P^T over a tile of codes, V's scales in P: a bf16 high part and the
+        // remainder, 16 bits together as long as p * 2^e stays above 2^-110.  Of rows whose
+        // largest value is below 2^-86 the smallest weights lose some of them, at most 2^-117
+        // of the result for each row.
         __device__ __forceinline__ void pv_codes(const unsigned char *v_lds, const int (&v_off)[kAttD / 32], const bf16x8_t (&phi)[1][2],
                                                  const bf16x8_t (&plo)[1][2], f32x16_t (&o)[kAttD / 32])
         {

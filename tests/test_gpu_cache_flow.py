@@ -1,6 +1,6 @@
 """The 8-bit KV cache and the speculative operators run together, as a serving loop does: ragged decode steps captured in
 a graph and replayed while the lengths grow on the device, a speculative step on a stream of its own, two graphs that share
-a workspace, and caches past 4 GiB."""
+a workspace, two calls at once, and caches past 4 GiB."""
 import numpy as np
 import pytest
 
@@ -190,6 +190,46 @@ def test_two_graphs_share_a_workspace(q3k, hip):
     finally:
         for g in graphs:
             g.destroy()
+
+
+def test_two_calls_at_once(q3k, hip):
+    """Split calls on two streams, each with a workspace of its own, give what they give alone."""
+    announce("two calls at once")
+    B, Hq, Hkv, cached, T = 1, 16, 2, 4000, 6
+    rng = np.random.default_rng(9)
+    s = _Serving(hip, B, Hkv, cached, [cached] * B)
+    up = hip.DeviceBuffer.from_array
+    bk, bv = up(_normal(rng, B, cached, Hkv, D)), up(_normal(rng, B, cached, Hkv, D))
+    q3k.kv_append_e4m3(bk, bv, s.kc, s.vc, s.sc, B, cached, Hkv, D, cached, 0)
+    parents = up(np.arange(-1, T - 1, dtype=np.int32))
+    q = [up(_normal(rng, B, S, Hq, D, std=2.0)) for S in (1, T)]
+    size = [q3k.cache_attention_workspace_bytes(B, S, Hq, Hkv, D, cached) for S in (1, T)]
+    assert min(size) > 0
+    ws = [hip.DeviceBuffer(n) for n in size]
+    streams = [hip.Stream() for _ in range(2)]
+
+    def call(i, out, stream):
+        kw = dict(stream=stream, workspace=ws[i], workspace_bytes=size[i])
+        if i == 0:
+            q3k.gqa_attention_e4m3(q[0], s.kc, s.vc, s.sc, out, B, 1, Hq, Hkv, D, cached, cached, **kw)
+        else:
+            q3k.gqa_tree_attention_e4m3(q[1], s.kc, s.vc, s.sc, out, parents, 0, B, T, Hq, Hkv, D, cached, cached, **kw)
+
+    shapes = [(B, 1, Hq, D), (B, T, Hq, D)]
+    outs = [[hip.DeviceBuffer(int(np.prod(shape)) * 2) for _ in range(20)] for shape in shapes]
+    alone = [hip.DeviceBuffer(int(np.prod(shape)) * 2) for shape in shapes]
+    hip.synchronize()
+    for i in range(2):
+        call(i, alone[i], None)
+        hip.synchronize()
+    for n in range(20):
+        for i in range(2):
+            call(i, outs[i][n], streams[i])
+    for stream in streams:
+        stream.synchronize()
+    for i, shape in enumerate(shapes):
+        want = alone[i].download(np.uint16, shape)
+        assert all(np.array_equal(o.download(np.uint16, shape), want) for o in outs[i])
 
 
 def test_rows_past_4_gib(q3k, hip):

@@ -433,3 +433,43 @@ def test_keep_path_scalar_start_of_a_long_path(q3k, hip):
     want[:, 0, :, 50:150] = k[:, 0, :, 50:250:2]
     for b in (bk, bv):
         assert np.array_equal(b.get(np.uint8, k.shape), want) and b.guards_intact()
+
+
+def test_keep_path_starts_and_counts_out_of_range(q3k, hip):
+    """A start outside the cache or a count below 0 leaves a sequence alone, a count past the path ends with it."""
+    announce("kv_keep_path starts and counts out of range")
+    B, seq, n = 8, 20, 3
+    k = np.random.default_rng(5).integers(0, 256, (2, B, 2, seq, 128), dtype=np.uint8)
+    s = np.random.default_rng(6).integers(0, 256, (2, B, 2, seq, 2), dtype=np.uint8)
+    starts = np.array([-1, LOWEST, HIGHEST, HIGHEST - 1, 20, 17, 4, 6], np.int32)
+    counts = np.array([n, n, n, n, n, n, -1, HIGHEST], np.int32)
+    path = np.tile(np.array([2, 3, HIGHEST], np.int32), (B, 1))
+    path[7] = [1, 1, 4]
+    bk, bv, bs = Guarded(hip, k), Guarded(hip, k), Guarded(hip, s)
+    bp, bst, bc = _up(hip, path, starts, counts)
+    q3k.kv_keep_path(bk, bv, bs, 2, B, 2, seq, 128, B, 0, bp, n, starts=bst, counts=bc)
+    hip.synchronize()
+    for bufs, a in (((bk, bv), k), ((bs,), s)):
+        want = a.copy()
+        want[:, 5, :, 17] = a[:, 5, :, 19]              # row 17 + 3 lies past the cache
+        want[:, 7, :, 6], want[:, 7, :, 8] = a[:, 7, :, 7], a[:, 7, :, 10]
+        for b in bufs:
+            assert np.array_equal(b.get(np.uint8, a.shape), want) and b.guards_intact()
+
+
+@pytest.mark.parametrize("S", [1, 40])
+def test_small_and_large_values(q3k, hip, S):
+    """Rows of 2^-60 to 2^60 in one cache: each row's scale is its own."""
+    def edit(c):
+        powers = np.exp2(np.random.default_rng(8).integers(-60, 61, (c.values[1].shape[0], c.cap, 1, 1)).astype(float))
+        rows = c.values[1] * powers                     # V of each row scaled by a power of two: codes stay, bytes move
+        finite = np.isfinite(rows)
+        c.values[1] = np.where(finite, rows, c.values[1])
+        move = np.log2(powers[..., 0, 0]).astype(int)
+        for b in range(c.bytes.shape[0]):
+            for row in range(c.cap):
+                byte = c.bytes[b, :, row, 1].astype(int)
+                c.bytes[b, :, row, 1] = np.where(byte < 255, byte + move[b, row], 255)
+        c.upload()
+
+    _compare(q3k, hip, f"values of 2^-60 to 2^60 S {S}", True, 2, S, 4, 2, 128, 90, 88, [88, 57], edit=edit)
