@@ -144,52 +144,46 @@ namespace q3k
                 scales[2 * at + l] = static_cast<uint8_t>(l == 0 ? sk : sv);
         }
 
-        // kReadPositions positions of a sequence a lane, all their codes before the stores:
-        // a head's positions lie together in the cache.  Groups of G lanes run over the heads
-        // first, so that a wave's stores cover whole positions.
-        // 16 x 4096 positions of 8 heads: 71.5 us, 404 MB at 5.65 TB/s (76.2 with four
-        // positions, 84.4 with eight).  Of ragged sequences four were between 5% faster and
-        // 12% slower, and slower wherever the call was small.
-        constexpr int kReadPositions = 2;
+        // Two heads of a position a lane (h and h + half of them), the codes of both before
+        // the stores, so that the groups of G lanes of a wave store one run of rows and then
+        // the run behind it.  16 x 4096 positions of 8 heads: 67.7 us, 404 MB at 5.96 TB/s; of
+        // ragged sequences 44.3 us.  With two positions of a head a lane instead 68.0 to 72.7
+        // and 44.2 to 48.1, with four positions 71.5 to 76.2 and 45.9 to 47.4; with rows in
+        // the output's order whatever their heads 67.3 to 68.5 and 44.0 to 48.6.
+        constexpr int kReadHeads = 2;
 
         template <int G>
         __global__ __launch_bounds__(kBlock) void read_rows_kernel(const uint8_t *__restrict__ kc, const uint8_t *__restrict__ vc,
                                                                    const uint8_t *__restrict__ scales, Vec8 *__restrict__ k,
-                                                                   Vec8 *__restrict__ v, E4m3Shape s, uint32_t steps)
+                                                                   Vec8 *__restrict__ v, E4m3Shape s)
         {
-            // unit: (sequence, step of positions, head)
-            const uint32_t unit = blockIdx.x * (kBlock / G) + threadIdx.x / G;
-            const uint32_t bp = unit / s.Hkv, h = unit - bp * s.Hkv;
-            const uint32_t b = bp / steps, p0 = (bp - b * steps) * kReadPositions;
-            if (b >= s.rows / (s.S * s.Hkv))
+            // unit: (sequence, position, head of the first half)
+            const uint32_t half = (s.Hkv + kReadHeads - 1) / kReadHeads;
+            const uint32_t unit = blockIdx.x * (kBlock / G) + threadIdx.x / G, l = threadIdx.x % G;
+            const uint32_t token = unit / half, h0 = unit - token * half;
+            const uint32_t b = token / s.S;
+            const int64_t pos = s.start + (token - b * s.S);
+            if (token >= s.rows / s.Hkv || (s.starts != nullptr && pos >= s.starts[b]))
                 return;
-            const uint32_t l = threadIdx.x % G;
-            // positions of this sequence that are read, counted from start
-            int64_t n = s.S;
-            if (s.starts != nullptr)
-                n = s.starts[b] - s.start < n ? s.starts[b] - s.start : n;
-            const int64_t at = cache_row(s, b, h, s.start + p0);
-            const uint2 *kp = reinterpret_cast<const uint2 *>(kc) + at * G + l, *vp = reinterpret_cast<const uint2 *>(vc) + at * G + l;
-            const uint8_t *sp = scales + 2 * at;
-            uint2 ck[kReadPositions], cv[kReadPositions];
-            uint32_t sk[kReadPositions], sv[kReadPositions];
+            uint2 ck[kReadHeads], cv[kReadHeads];
+            uint32_t sk[kReadHeads], sv[kReadHeads];
 #pragma unroll
-            for (int u = 0; u < kReadPositions; ++u)
-                if (p0 + u < n)
+            for (int x = 0; x < kReadHeads; ++x)
+                if (h0 + x * half < s.Hkv)
                 {
-                    ck[u] = kp[u * G];
-                    cv[u] = vp[u * G];
-                    sk[u] = sp[2 * u];
-                    sv[u] = sp[2 * u + 1];
+                    const int64_t at = cache_row(s, b, h0 + x * half, pos);
+                    ck[x] = reinterpret_cast<const uint2 *>(kc)[at * G + l];
+                    cv[x] = reinterpret_cast<const uint2 *>(vc)[at * G + l];
+                    sk[x] = scales[2 * at];
+                    sv[x] = scales[2 * at + 1];
                 }
-            const int64_t row0 = (static_cast<int64_t>(b) * s.S + p0) * s.Hkv + h;
 #pragma unroll
-            for (int u = 0; u < kReadPositions; ++u)
-                if (p0 + u < n)
+            for (int x = 0; x < kReadHeads; ++x)
+                if (h0 + x * half < s.Hkv)
                 {
-                    const int64_t out = (row0 + static_cast<int64_t>(u) * s.Hkv) * G + l;
-                    store8<kStoreStream>(k + out, decode8(ck[u], e4m3_scale(sk[u])));
-                    store8<kStoreStream>(v + out, decode8(cv[u], e4m3_scale(sv[u])));
+                    const int64_t out = (static_cast<int64_t>(token) * s.Hkv + h0 + x * half) * G + l;
+                    store8<kStoreStream>(k + out, decode8(ck[x], e4m3_scale(sk[x])));
+                    store8<kStoreStream>(v + out, decode8(cv[x], e4m3_scale(sv[x])));
                 }
         }
 
@@ -334,14 +328,12 @@ extern "C" int q3k_kv_read_e4m3_bf16(const uint8_t *k_codes, const uint8_t *v_co
     Vec8 *k = reinterpret_cast<Vec8 *>(key), *v = reinterpret_cast<Vec8 *>(value);
     const dim3 block(kBlock);
     const int lanes = row_lanes(s, aligned16(key) && aligned16(value) && aligned_to(k_codes, 8) && aligned_to(v_codes, 8));
-    const int64_t steps = blocks_for(count, kReadPositions);
-    const dim3 grid(lanes == 0 ? generic_grid(s) : static_cast<unsigned>(blocks_for(B * steps * Hkv, kBlock / lanes)));
-    const uint32_t st32 = static_cast<uint32_t>(steps);
+    const dim3 grid(lanes == 0 ? generic_grid(s) : static_cast<unsigned>(blocks_for(B * count * blocks_for(Hkv, kReadHeads), kBlock / lanes)));
     switch (lanes)
     {
-    case 8: read_rows_kernel<8><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
-    case 16: read_rows_kernel<16><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
-    case 32: read_rows_kernel<32><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s, st32); break;
+    case 8: read_rows_kernel<8><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
+    case 16: read_rows_kernel<16><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
+    case 32: read_rows_kernel<32><<<grid, block, 0, st>>>(k_codes, v_codes, scales, k, v, s); break;
     default: read_generic_kernel<<<grid, block, 0, st>>>(k_codes, v_codes, scales, key, value, s); break;
     }
     return check_launch("kv_read_e4m3");
