@@ -884,10 +884,11 @@ namespace q3k
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
             // KV heads run fastest, so that with a multiple of 8 of them the blocks of a pair
-            // meet on one XCD, whose L2 holds its K and V.  A tree's query blocks are equally
-            // long: sequences outermost; but a last block of fewer columns is lighter, and
-            // those come after all others.  Causal ones differ: slices
-            // outermost, then the query blocks, longest first, then the sequences.
+            // meet on one XCD, whose L2 holds its K and V.  Slices outermost: those of whole
+            // length first, and a CU's two blocks are of different ones (6 trees of 200 nodes
+            // over up to 5000 rows in 4 slices 74 us, 112 with a sequence's slices side by
+            // side).  A tree's query blocks are equally long, but a last one of fewer columns
+            // is lighter, and those come after all others; causal ones go longest first.
             int32_t sp, qb, kvh;
             int64_t b;
             if constexpr (TREE)
@@ -899,8 +900,8 @@ namespace q3k
                 const int32_t light = unit - a.B * a.splits * whole;
                 qb = light >= 0 ? whole : unit % whole;
                 unit = light >= 0 ? light : unit / whole;
-                sp = unit % a.splits;
-                b = unit / a.splits;
+                sp = unit / a.B;
+                b = unit - sp * a.B;
             }
             else
             {

@@ -529,7 +529,7 @@ namespace q3k
     // and 0.81 us (1.54) of CU time where blocks queue or share a CU; a query block that is
     // not full costs 0.64 of a full one and its columns' part of the rest; start and end 9.8
     // us (4.7).  Causal query blocks see between cached - S and cached rows.  Fitted to 550
-    // shapes of 1 to 100 sequences and 12 to 400 queries or nodes: 1.0% slower than the best
+    // shapes of 1 to 100 sequences and 12 to 400 queries or nodes: 0.8% slower than the best
     // of the one to twenty forms of each on average, 26% at worst.
     inline double cache_block_us(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int64_t cached, bool e4m3, bool tree, bool ragged,
                                  int key_groups, int64_t split_keys)
