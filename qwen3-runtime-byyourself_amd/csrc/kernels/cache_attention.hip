@@ -95,10 +95,11 @@ namespace q3k
         // given; the whole wave calls it.  Decode blocks take sequences of different lengths
         // longest first, so that what starts last is short (64 of 1024 to 4096 rows, 8 KV
         // heads: 66.4 us, 78.0 in a random order; of 4000 to 16000 rows 231 us and 278; their
-        // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  In the block kernels,
-        // two blocks to a CU, it gave nothing (16 trees of 64 nodes, 40 heads: 124 to 130 us,
-        // 122 in a random order).  Of more than 64 sequences each 64 are ordered among
-        // themselves.
+        // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  Ranking them takes
+        // 1.5 us, more than it gives sequences that are cut into slices (4 of up to 8000 rows:
+        // 17.4 us, 19.1 ordered).  In the block kernels, two blocks to a CU, it gave nothing
+        // (16 trees of 64 nodes, 40 heads: 124 to 130 us, 122 in a random order).  Of more
+        // than 64 sequences each 64 are ordered among themselves.
         __device__ __forceinline__ int32_t sequence_at(const CacheArgs &a, int32_t rank, int lane)
         {
             if (!a.ordered)
@@ -625,8 +626,10 @@ namespace q3k
             const int kw = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
             const int lane = threadIdx.x % kWave;
             const int li = lane % 32, lg = lane / 32;
-            // slices of a pair side by side
-            const int32_t sp = static_cast<int32_t>(blockIdx.x) % a.splits, pair = static_cast<int32_t>(blockIdx.x) / a.splits;
+            // Slices outermost: those of whole length first, each spread over the XCDs (4
+            // sequences of up to 8000 rows 17.2 us, 19.1 with a pair's slices side by side).
+            const int32_t pairs = a.B * a.Hkv;
+            const int32_t sp = static_cast<int32_t>(blockIdx.x) / pairs, pair = static_cast<int32_t>(blockIdx.x) - sp * pairs;
             const int32_t kvh = pair % a.Hkv;
             const int64_t b = sequence_at(a, pair / a.Hkv, lane);
             const int32_t S = static_cast<int32_t>(a.S);
