@@ -104,19 +104,25 @@ namespace q3k
         {
             if (!a.ordered)
                 return rank;
-            const int32_t first = rank / kWave * kWave;
-            // equal lengths in the order given; lanes past the last sequence come last, also
-            // behind lengths below 0, which are errors but have a place
-            const int32_t length = first + lane < a.B ? a.lengths[first + lane] : 0;
-            const int32_t n = first + lane < a.B ? (length > 0 ? length : 0) : -1;
-            uint32_t before = 0;
-#pragma unroll
-            for (int i = 0; i < kWave; ++i)
+            const int32_t first = rank / kWave * kWave, r = rank - first;
+            // lengths past the cache's count as one more, those below 0 as 0 (errors, but they
+            // have a place); lanes past the last sequence come last
+            const int32_t most = static_cast<int32_t>(a.cached) + 1;
+            int32_t n = first + lane < a.B ? a.lengths[first + lane] : -1;
+            n = first + lane >= a.B ? -1 : n < 0 ? 0 : n > most ? most : n;
+            // the r-th largest, bit by bit, and of those that have it the one whose turn it is
+            // by the order given
+            int32_t value = 0;
+            for (int bit = 31 - __builtin_clz(static_cast<uint32_t>(most)); bit >= 0; --bit)
             {
-                const int32_t other = __builtin_amdgcn_readlane(n, i);
-                before += (other > n) || (other == n && i < lane) ? 1u : 0u;
+                const int32_t with = value | 1 << bit;
+                value = __builtin_popcountll(__ballot(n >= with)) > r ? with : value;
             }
-            return first + static_cast<int32_t>(__builtin_ctzll(__ballot(before == static_cast<uint32_t>(rank - first))));
+            const uint64_t equal = __ballot(n == value);
+            const int32_t turn = r - __builtin_popcountll(__ballot(n > value));
+            const int32_t before = static_cast<int32_t>(__builtin_amdgcn_mbcnt_hi(
+                static_cast<uint32_t>(equal >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(equal), 0)));
+            return first + static_cast<int32_t>(__builtin_ctzll(__ballot(n == value && before == turn)));
         }
 
         // Walks up from node t and calls visit(u) for the node and each ancestor.
