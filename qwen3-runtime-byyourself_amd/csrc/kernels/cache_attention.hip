@@ -95,9 +95,9 @@ namespace q3k
         // given; the whole wave calls it.  Decode blocks take sequences of different lengths
         // longest first, so that what starts last is short (64 of 1024 to 4096 rows, 8 KV
         // heads: 66.4 us, 78.0 in a random order; of 4000 to 16000 rows 231 us and 278; their
-        // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  Ranking them takes
-        // 1.5 us, more than it gives sequences that are cut into slices (4 of up to 8000 rows:
-        // 17.4 us, 19.1 ordered).  In the block kernels, two blocks to a CU, it gave nothing
+        // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  Finding the
+        // place takes 0.6 to 1 us, more than it gives sequences that are cut into slices (4 of
+        // up to 8000 rows: 17.3 us, 18.4 ordered).  In the block kernels, two blocks to a CU, it gave nothing
         // (16 trees of 64 nodes, 40 heads: 124 to 130 us, 122 in a random order).  Of more
         // than 64 sequences each 64 are ordered among themselves.
         __device__ __forceinline__ int32_t sequence_at(const CacheArgs &a, int32_t rank, int lane)
