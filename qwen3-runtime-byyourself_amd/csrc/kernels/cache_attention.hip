@@ -62,14 +62,17 @@ namespace q3k
             int64_t rows;
             int32_t B;
             bool ordered; // decode blocks take the sequences longest first
-            // the fast kernels: query blocks of a pair, slices of split_keys rows, their
-            // results (unnormalised O^T [splits, rows, D], reference max and sum
-            // [splits, rows, 2])
+            // the fast kernels: query heads of a KV head, query blocks of a pair, slices of
+            // split_keys rows, their results (unnormalised O^T [splits, rows, D], reference max
+            // and sum [splits, rows, 2])
+            int32_t g;
             int32_t qblocks;
             int32_t splits;
             int32_t split_keys;
             float *part_o;
             float *part_ml;
+            // by (sequence, KV head) pairs; by query blocks, of a tree by those of all their columns
+            Divisor by_g, by_hkv, by_pairs, by_b, by_qblocks;
         };
 
         constexpr int kTreeWords = kTreeMaxNodes / 64;
@@ -587,12 +590,11 @@ namespace q3k
         __device__ __forceinline__ void fill_columns(const CacheArgs &a, int64_t b, int kvh, int32_t col0, int32_t col_end, bool nan,
                                                      int thread, int threads)
         {
-            const int g = a.Hq / a.Hkv;
             const uint32_t w = nan ? 0x7fc07fc0u : 0u;
             for (int32_t i = thread; i < (col_end - col0) * (kAttD / 4); i += threads)
             {
                 const int32_t col = col0 + i / (kAttD / 4);
-                const int64_t row = (b * a.S + col / g) * a.Hq + kvh * g + col % g;
+                const int64_t row = (b * a.S + col / a.by_g) * a.Hq + kvh * a.g + col % a.by_g;
                 reinterpret_cast<uint2 *>(a.out + row * kAttD)[i % (kAttD / 4)] = make_uint2(w, w);
             }
         }
@@ -634,12 +636,11 @@ namespace q3k
             const int li = lane % 32, lg = lane / 32;
             // Slices outermost: those of whole length first, each spread over the XCDs (4
             // sequences of up to 8000 rows 17.2 us, 19.1 with a pair's slices side by side).
-            const int32_t pairs = a.B * a.Hkv;
-            const int32_t sp = static_cast<int32_t>(blockIdx.x) / pairs, pair = static_cast<int32_t>(blockIdx.x) - sp * pairs;
-            const int32_t kvh = pair % a.Hkv;
-            const int64_t b = sequence_at(a, pair / a.Hkv, lane);
+            const int32_t sp = static_cast<int32_t>(blockIdx.x) / a.by_pairs, pair = static_cast<int32_t>(blockIdx.x) % a.by_pairs;
+            const int32_t kvh = pair % a.by_hkv;
+            const int64_t b = sequence_at(a, pair / a.by_hkv, lane);
             const int32_t S = static_cast<int32_t>(a.S);
-            const int g = a.Hq / a.Hkv;
+            const int g = a.g;
             bool bad;
             const int32_t n_keys = sequence_rows(a, b, bad);
             if (n_keys == 0)
@@ -663,8 +664,8 @@ namespace q3k
             if constexpr (TREE)
                 parent = a.parents[b * a.parents_stride + (lane < S ? lane : S - 1)];
             // the lane's column; lanes past the last one repeat a row of the last position
-            const int32_t s_col = li / g;
-            const int h_col = kvh * g + li % g;
+            const int32_t s_col = li / a.by_g;
+            const int h_col = kvh * g + li % a.by_g;
             const bool col_ok = s_col < S;
             const int32_t s_row = col_ok ? s_col : S - 1;
 
@@ -871,7 +872,7 @@ namespace q3k
         template <int CW, int KW, int HH, bool E4M3, bool TREE>
         __global__ __launch_bounds__(CW *KW *kWave, 2) void cache_block_kernel(CacheArgs a)
         {
-            const int g = a.Hq / a.Hkv;
+            const int g = a.g;
             constexpr int kBlockCols = 32 * CW;
             constexpr int kKeys = 32 * HH;
             constexpr int kTileBytes = kKeys * kRowBytes;
@@ -903,29 +904,28 @@ namespace q3k
             if constexpr (TREE)
             {
                 int32_t unit = static_cast<int32_t>(blockIdx.x);
-                kvh = unit % a.Hkv;
-                unit /= a.Hkv;
-                const int32_t whole = static_cast<int32_t>(a.S) * g / kBlockCols; // query blocks of all their columns
+                kvh = unit % a.by_hkv;
+                unit = unit / a.by_hkv;
+                const int32_t whole = static_cast<int32_t>(a.S) * g / kBlockCols;
                 const int32_t light = unit - a.B * a.splits * whole;
-                qb = light >= 0 ? whole : unit % whole;
-                unit = light >= 0 ? light : unit / whole;
-                sp = unit / a.B;
-                b = unit - sp * a.B;
+                qb = light >= 0 ? whole : unit % a.by_qblocks;
+                unit = light >= 0 ? light : unit / a.by_qblocks;
+                sp = unit / a.by_b;
+                b = unit % a.by_b;
             }
             else
             {
-                const int32_t pairs = static_cast<int32_t>(gridDim.x) / (a.qblocks * a.splits);
-                const int32_t pair = static_cast<int32_t>(blockIdx.x) % pairs, rest = static_cast<int32_t>(blockIdx.x) / pairs;
-                sp = rest / a.qblocks;
-                qb = a.qblocks - 1 - rest % a.qblocks;
-                kvh = pair % a.Hkv;
-                b = pair / a.Hkv;
+                const int32_t pair = static_cast<int32_t>(blockIdx.x) % a.by_pairs, rest = static_cast<int32_t>(blockIdx.x) / a.by_pairs;
+                sp = rest / a.by_qblocks;
+                qb = a.qblocks - 1 - rest % a.by_qblocks;
+                kvh = pair % a.by_hkv;
+                b = pair / a.by_hkv;
             }
             const int32_t S = static_cast<int32_t>(a.S);
             const int32_t n_cols = S * g;
             const int32_t block_col = qb * kBlockCols;
             const int32_t block_end = n_cols - block_col > kBlockCols ? block_col + kBlockCols : n_cols;
-            const int32_t s_first = block_col / g, s_last = (block_end - 1) / g;
+            const int32_t s_last = (block_end - 1) / a.by_g;
             bool bad;
             const int32_t n = sequence_rows(a, b, bad);
             const int32_t context = n - S;
@@ -961,12 +961,12 @@ namespace q3k
             const int32_t wave_col = block_col + 32 * cw;
             const int32_t col = wave_col + li;
             const bool col_ok = col < n_cols;
-            const int32_t s_col = col / g;
-            const int h_col = kvh * g + col % g;
+            const int32_t s_col = col / a.by_g;
+            const int h_col = kvh * g + col % a.by_g;
             const int32_t s_row = col_ok ? s_col : S - 1;
             const bool wave_active = wave_col < n_cols;
             // rows that every query of the wave sees
-            const int32_t all_seen = TREE ? context : context + wave_col / g + 1;
+            const int32_t all_seen = TREE ? context : context + wave_col / a.by_g + 1;
 
             constexpr int64_t kElement = E4M3 ? 1 : 2;
             const unsigned char *kbase = static_cast<const unsigned char *>(a.k) + (b * a.ks0 + kvh * a.ks2) * kElement;
@@ -1212,14 +1212,19 @@ namespace q3k
 
         // ---- merging slices ---------------------------------------------------------------
 
+        struct MergeShape
+        {
+            Divisor by_hq, by_s, by_split_keys;
+            int32_t last_col; // of a query block (its columns are a power of two)
+        };
+
         // How many slices hold a query row's keys; 0: its query block wrote the result.
         // With several positions a row takes the slices its own keys reach (in the others of
         // its query block all its scores are masked).
-        __device__ __forceinline__ int row_slices(const CacheArgs &a, int64_t row, int32_t block_cols)
+        __device__ __forceinline__ int row_slices(const CacheArgs &a, const MergeShape &m, int64_t row)
         {
-            const uint32_t r32 = static_cast<uint32_t>(row), hq = static_cast<uint32_t>(a.Hq), S = static_cast<uint32_t>(a.S);
-            const uint32_t bs = r32 / hq, h = r32 - bs * hq, b = bs / S;
-            const int32_t s = static_cast<int32_t>(bs - b * S);
+            const int32_t r32 = static_cast<int32_t>(row), bs = r32 / m.by_hq, h = r32 - bs * a.Hq, b = bs / m.by_s;
+            const int32_t s = bs - b * static_cast<int32_t>(a.S);
             bool bad;
             const int32_t n = sequence_rows(a, b, bad);
             if (n == 0)
@@ -1227,13 +1232,12 @@ namespace q3k
             int32_t own = n, block = n; // rows that this query's slices and its block's reach
             if (a.parents == nullptr)
             {
-                const int32_t g = a.Hq / a.Hkv, col = s * g + static_cast<int32_t>(h) % g;
-                const int64_t last = ((static_cast<int64_t>(col) / block_cols + 1) * block_cols - 1) / g;
-                const int32_t s_last = last < a.S ? static_cast<int32_t>(last) : static_cast<int32_t>(a.S) - 1;
+                const int32_t col = s * a.g + h % a.by_g, last = (col | m.last_col) / a.by_g;
+                const int32_t s_last = last < a.S ? last : static_cast<int32_t>(a.S) - 1;
                 own = n - static_cast<int32_t>(a.S) + s + 1;
                 block = own + s_last - s;
             }
-            return block <= a.split_keys ? 0 : own <= 0 ? 1 : (own - 1) / a.split_keys + 1;
+            return block <= a.split_keys ? 0 : own <= 0 ? 1 : (own - 1) / m.by_split_keys + 1;
         }
 
         // Few rows, many slices: a block of four waves a row (32 rows of 32 slices 2.8 us,
@@ -1243,13 +1247,13 @@ namespace q3k
         constexpr int kMergeWaves = 4;
         constexpr int kMergeRound = kAttMaxSplits / kMergeWaves;
 
-        __global__ __launch_bounds__(kMergeWaves *kWave) void cache_merge_block_kernel(CacheArgs a, int32_t block_cols)
+        __global__ __launch_bounds__(kMergeWaves *kWave) void cache_merge_block_kernel(CacheArgs a, MergeShape shape)
         {
             __shared__ float2 wave_acc[kMergeWaves][kWave];
             const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
             const int lane = threadIdx.x % kWave;
             const int64_t row = blockIdx.x;
-            const int slices = row_slices(a, row, block_cols);
+            const int slices = row_slices(a, shape, row);
             if (slices == 0)
                 return;
             float2 ml = make_float2(-__builtin_huge_valf(), 0.0f);
@@ -1302,12 +1306,12 @@ namespace q3k
         constexpr int kMergeSlices = 4;
         constexpr int kMergeRows = kBlock / 16;
 
-        __global__ __launch_bounds__(kBlock) void cache_merge_rows_kernel(CacheArgs a, int32_t block_cols)
+        __global__ __launch_bounds__(kBlock) void cache_merge_rows_kernel(CacheArgs a, MergeShape shape)
         {
             const int64_t row = static_cast<int64_t>(blockIdx.x) * kMergeRows + threadIdx.x / 16;
             if (row >= a.rows)
                 return;
-            const int slices = row_slices(a, row, block_cols), d = 8 * (threadIdx.x % 16);
+            const int slices = row_slices(a, shape, row), d = 8 * (threadIdx.x % 16);
             if (slices == 0)
                 return;
             float mx = -__builtin_huge_valf(), lsum = 0.0f, acc[8] = {};
@@ -1353,11 +1357,11 @@ namespace q3k
         {
             if (a.splits > 1)
             {
+                const MergeShape m{divisor(a.Hq), divisor(a.S), divisor(a.split_keys), block_cols - 1};
                 if (a.rows <= kAttBlockMergeRows)
-                    cache_merge_block_kernel<<<dim3(static_cast<unsigned>(a.rows)), dim3(kMergeWaves * kWave), 0, stream>>>(a, block_cols);
+                    cache_merge_block_kernel<<<dim3(static_cast<unsigned>(a.rows)), dim3(kMergeWaves * kWave), 0, stream>>>(a, m);
                 else
-                    cache_merge_rows_kernel<<<dim3(static_cast<unsigned>(blocks_for(a.rows, kMergeRows))), dim3(kBlock), 0, stream>>>(
-                        a, block_cols);
+                    cache_merge_rows_kernel<<<dim3(static_cast<unsigned>(blocks_for(a.rows, kMergeRows))), dim3(kBlock), 0, stream>>>(a, m);
             }
             return check_launch(what);
         }
@@ -1376,7 +1380,9 @@ namespace q3k
         int launch_block(const char *what, CacheArgs a, int64_t B, hipStream_t stream)
         {
             constexpr int kBlockCols = 32 * CW, kThreads = CW * KW * kWave;
-            a.qblocks = static_cast<int32_t>(blocks_for(a.S * (a.Hq / a.Hkv), kBlockCols));
+            a.qblocks = static_cast<int32_t>(blocks_for(a.S * a.g, kBlockCols));
+            const int64_t whole = a.S * a.g / kBlockCols;
+            a.by_qblocks = divisor(!TREE ? a.qblocks : whole > 0 ? whole : 1);
             const int64_t blocks = B * a.Hkv * a.qblocks * a.splits;
             if (!launch_fits(blocks, kThreads) || blocks > INT32_MAX)
                 return set_error(Q3K_ERR_OVERFLOW, "%s grid is too large", what);
@@ -1491,6 +1497,11 @@ namespace q3k
                 a.ordered = ragged && B > 1 && p.splits == 1 && p.decode_waves > 0;
                 a.splits = p.splits;
                 a.split_keys = p.split_keys;
+                a.g = a.Hq / a.Hkv;
+                a.by_g = divisor(a.g);
+                a.by_hkv = divisor(a.Hkv);
+                a.by_b = divisor(B);
+                a.by_pairs = divisor(B * a.Hkv);
                 a.part_o = static_cast<float *>(workspace);
                 a.part_ml = p.splits > 1 ? a.part_o + static_cast<int64_t>(p.splits) * a.rows * kAttD : nullptr;
                 if (tree)

@@ -1,7 +1,7 @@
 // The plans of the attention over a cache with a length for each sequence
 // (csrc/kernels/dispatch.hpp): a workspace sized for the cache's length holds the
 // slices of every shorter one, slices are whole tiles and few enough to merge,
-// and a call that may not cut its keys does not.
+// and a call that may not cut its keys does not; and the kernels' divisions.
 #include "../../qwen3-runtime-byyourself_amd/csrc/kernels/dispatch.hpp"
 #include "test_util.hpp"
 
@@ -11,9 +11,29 @@ using test::require;
 
 namespace
 {
+    // x / d by the kernels' multiplication, at and around multiples of d up to 2^31 - 1.
+    void divisions()
+    {
+        using namespace q3k;
+        for (int64_t d = 1; d <= INT32_MAX; d += d < 3000 ? 1 : d / 7)
+            for (const int64_t by : {d - 1, d, d + 1})
+            {
+                if (by < 1 || by > INT32_MAX)
+                    continue;
+                const Divisor v = divisor(by);
+                for (int64_t q = 0; q * by <= INT32_MAX; q += 1 + q / 5)
+                    for (const int64_t x : {q * by - 1, q * by, q * by + 1, q * by + by / 2})
+                        if (x >= 0 && x <= INT32_MAX)
+                            require(static_cast<int32_t>(x) / v == x / by && static_cast<int32_t>(x) % v == x % by,
+                                    std::to_string(x) + " / " + std::to_string(by));
+                require(INT32_MAX / v == INT32_MAX / by, "2^31 - 1 / " + std::to_string(by));
+            }
+    }
+
     void body()
     {
         using namespace q3k;
+        divisions();
         const int32_t heads[][2] = {{16, 8}, {32, 8}, {40, 8}, {64, 8}, {2, 1}, {4, 1}, {5, 1}, {8, 1}, {32, 1}};
         int64_t cut = 0, whole = 0, waves[9] = {};
         for (const auto &h : heads)
