@@ -615,9 +615,9 @@ namespace q3k
         // the keys are long (8 sequences of 1000 rows whole: 12.9 us, 15.8 with KW 4; 32
         // ragged ones of up to 2500 29.7 and 38.4), else of two (64 of up to 1000: 23.3 us,
         // 28.0 with KW 8).
-        // 64 ragged sequences of 1024 to 4096 rows, 32 / 8 heads: 66 to 73 us, 339 MB at 4.7
-        // to 5.1 TB/s of the 5.4 to 5.9 that the access pattern reaches; one of 8191 rows,
-        // 16 / 8 heads, cut into slices, 11.4 us, of which the merge takes 2.8.
+        // 64 ragged sequences of 1024 to 4096 rows, 32 / 8 heads: 65 to 72 us, 339 MB at 4.7
+        // to 5.2 TB/s of the 5.4 to 5.9 that the access pattern reaches; one of 8191 rows,
+        // 16 / 8 heads, cut into slices, 10.8 us, of which the merge takes 2.8.
         template <int KW, bool E4M3, bool TREE>
         __global__ __launch_bounds__(KW *kWave, E4M3 ? 2 : 1) void cache_decode_kernel(CacheArgs a)
         {
@@ -863,10 +863,10 @@ namespace q3k
         //   registers for loads in flight (holding the codes in registers instead spilled
         //   or cost the second block of a CU).
         // What bounds it is the softmax beside the matrix instructions, as in the bf16
-        // attention.  512 queries over 8192 rows, 32 / 8 heads, e4m3, in 4 slices: 95 us and 8
-        // for the merge, 643 TFLOP/s of the products, matrix cores busy 44%.  16 ragged trees
-        // of 64 nodes over up to 4160 bf16 rows, 40 / 8 heads: 117 to 123 us, 440 to 455
-        // TFLOP/s, 384 blocks of unequal length, two to a CU.  Four groups with 64 columns
+        // attention.  512 queries over 8192 rows, 32 / 8 heads, e4m3, in 4 slices: 95 to 101 us
+        // and 8 for the merge, 590 to 640 TFLOP/s of the products, matrix cores busy 44%.  16
+        // ragged trees of 64 nodes over up to 4160 bf16 rows, 40 / 8 heads: 116 to 122 us, 440
+        // to 465 TFLOP/s, 384 blocks of unequal length, two to a CU.  Four groups with 64 columns
         // are for few blocks (4 trees of 64 nodes over 2000 rows: 38.4 us, 40.7 with 128
         // columns) and lose where there are many (64 of 16 nodes over 1000: 49.2 and 43.2).
         template <int CW, int KW, int HH, bool E4M3, bool TREE>
