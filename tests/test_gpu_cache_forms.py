@@ -1,0 +1,103 @@
+"""Every form of the attention over a cache (cache_forms) against the plain 64-bit form, at several tiles, query blocks and
+slices: finite values, and NaN in rows past the first tile that some queries see and others do not."""
+import numpy as np
+import pytest
+
+import cache_forms
+import cache_ref as ref
+from gpu_util import announce
+from test_gpu_cache_ops import _Cache, _queries, _random_trees, _run, _up, _workspace
+
+pytestmark = pytest.mark.gpu
+D = 128
+
+
+def _id(c):
+    return f"{c[0]}-{c[1]}x{c[2]}-{c[3]}.{c[4]}-{c[5]}{'r' if c[6] else ''}-{c[7].replace('/', 's')}"
+
+
+class _CodesCache(_Cache):
+    """An e4m3 cache of codes drawn as such (a normal distribution's), scale bytes of 2^-8 to 2^-6: about 1 in size."""
+
+    def __init__(self, hip, rng, B, Hkv, cap, lengths):
+        self.e4m3, self.cap, self.hip = True, cap, hip
+        pool = ref.encode(np.clip(rng.standard_normal(1 << 16) * 100, -448, 448))
+        past = (np.arange(cap)[None, :] >= np.asarray(lengths)[:, None])
+        self.bytes = rng.integers(119, 122, (B, Hkv, cap, 2), dtype=np.uint8)
+        self.values, self.stored = [], []
+        for i in range(2):
+            codes = pool[rng.integers(0, 1 << 16, (B, Hkv, cap, D), dtype=np.uint16)]
+            self.values.append(ref.dequantise(codes, self.bytes[..., i]).transpose(0, 2, 1, 3))
+            codes.transpose(0, 2, 1, 3)[past] = 0x7F
+            self.stored.append(codes)
+        self.bytes.transpose(0, 2, 1, 3)[past] = 255
+        self.upload()
+
+
+class _Call:
+    """One of cache_forms.FORMS with its inputs; rows of the cache past a sequence's length hold NaN."""
+
+    def __init__(self, hip, form, seed=0, edit=None):
+        self.hip = hip
+        kind, self.B, self.S, self.Hq, self.Hkv, self.cached, ragged = form[:7]
+        B, S = self.B, self.S
+        rng = np.random.default_rng(seed + B + 31 * S + self.cached)
+        self.lengths = cache_forms.lengths_of(B, S, self.cached, ragged)
+        self.n = np.full(B, self.cached) if self.lengths is None else self.lengths
+        if kind == "tree-bf16":
+            self.cache = _Cache(hip, rng, False, B, self.Hkv, D, self.cached + 3, self.n)
+        else:
+            self.cache = _CodesCache(hip, rng, B, self.Hkv, self.cached + 3, self.n)
+        self.trees = _random_trees(rng, B, S) if kind != "causal" else None
+        self.q = _queries(rng, B, S, self.Hq, D)
+        if edit is not None:
+            edit(self)
+        self.bq, = _up(hip, self.q)
+        self.bl = _up(hip, np.asarray(self.lengths, np.int32))[0] if ragged else None
+        self.bp = (_up(hip, self.trees)[0], S) if self.trees is not None else None
+
+    def shape(self):
+        return self.B, self.S, self.Hq, self.Hkv, D, self.cached
+
+    def run(self, q3k, ws):
+        out = _run(q3k, self.hip, self.cache, self.bq, self.B, self.S, self.Hq, self.Hkv, D, self.cached, self.bl, self.bp, ws)
+        self.hip.synchronize()
+        assert out.guards_intact() and (ws is None or ws[0].guards_intact())
+        return out.get(np.uint16, self.q.shape)
+
+    def want(self):
+        x = ref.bf16(self.q).reshape(self.q.shape)
+        k, v = self.cache.values
+        pairs = [cache_forms.attention(x[b], k[b, :n], v[b, :n], int(n), self.S, None if self.trees is None else self.trees[b])
+                 for b, n in enumerate(self.n)]
+        return np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs])
+
+
+def _check(q3k, hip, name, form, **kw):
+    announce(f"{name} {_id(form)}")
+    call = _Call(hip, form, **kw)
+    want = call.want()
+    ws = _workspace(q3k, hip, *call.shape())
+    for w in (None, ws) if ws is not None else (None,):
+        got = call.run(q3k, w)
+        ref.check_attention(f"{name} {_id(form)} workspace {w is not None}", got, *want)
+        assert np.array_equal(call.run(q3k, w), got), "a second call gives other bits"
+
+
+@pytest.mark.parametrize("form", cache_forms.FORMS, ids=_id)
+def test_form(q3k, hip, form):
+    _check(q3k, hip, "form", form)
+
+
+@pytest.mark.parametrize("form", [c for c in cache_forms.FORMS if c[2] > 1], ids=_id)
+def test_form_with_nan_rows(q3k, hip, form):
+    """K and V of a query's own row are NaN in half the sequences, in another tile in each (the lengths differ, or the
+    row): what does not see it is as if it were finite.  Of every third sequence a row of the context, which all see."""
+    def edit(call):
+        for b in range(0, call.B, 2):
+            call.cache.poison(b, int(call.n[b]) - call.S + (b + call.S // 2) % call.S)
+        for b in range(1, call.B, 3):
+            if call.n[b] > call.S + 70:
+                call.cache.poison(b, int(call.n[b]) - call.S - 1)
+
+    _check(q3k, hip, "NaN rows", form, seed=1, edit=edit)
