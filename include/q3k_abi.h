@@ -410,7 +410,9 @@ Q3K_API int q3k_gqa_attention_e4m3_bf16(const uint16_t *q, const uint8_t *k_code
  * not there (trees of different sizes in a batch): it and its descendants get
  * zeros.  A node whose way up meets any other number gets NaN, as does a
  * sequence whose length is neither 0 (zeros) nor in [T, cached].  What rows
- * hold that a node does not attend to, NaN included, does not reach it.
+ * hold that a node does not attend to, NaN included, does not reach it; an
+ * infinity of V in a row that it attends to (with a weight above 0) gives it
+ * that infinity, NaN where both signs meet.
  * k_cache / v_cache are views as those of q3k_gqa_attention_bf16, [B, cached,
  * Hkv, D] by element strides; `cached` and the workspace are as in
  * q3k_gqa_attention_e4m3_bf16; the fast kernels take head_dim 128 with unit dim

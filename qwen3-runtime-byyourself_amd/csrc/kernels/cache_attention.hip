@@ -25,7 +25,8 @@
 // what K holds in a row that a query does not see never counts.  What V holds there
 // meets a weight of zero, and zero times an infinity or a NaN is NaN: so a masked
 // tile is looked through for such values, and if there is one its product goes the
-// careful way (pv_careful).
+// careful way (pv_careful).  An infinity that a query does see is put right at the end
+// (see_infinities).
 //
 // Generic path (any head_dim <= 256, any strides and alignment): one wave per
 // query row, its rows in order, lanes over the head dimension, the running
@@ -526,6 +527,71 @@ namespace q3k
             return make_float4(bf_lo(lo), bf_hi(lo), bf_lo(hi), bf_hi(hi));
         }
 
+        // Infinities of V that a column does see.  A weight is a bf16 part and a remainder,
+        // and a remainder of zero, or below it, times an infinity is NaN, not the infinity.
+        // So where dims 32 dt .. + 31 of a result (elements of o as store_dims takes them)
+        // are not finite, the wave looks through rows begin .. end - 1 of V again and gives
+        // each such element the sum of the infinities and NaN that its column sees.  What
+        // they do not explain has left fp32's range, and stays infinite.  Only bf16 holds
+        // infinities.  Looking costs 16 instructions where all is finite, once a result.
+        template <typename Sees>
+        __device__ __forceinline__ void see_infinities(const unsigned char *vbase, int32_t vstride, int32_t begin, int32_t end,
+                                                       int dt, int lane, Sees sees, f32x16_t &o)
+        {
+            float zero = 0.0f; // NaN if one is not finite
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                zero = __builtin_fmaf(o[r], 0.0f, zero);
+            if (!__any(zero != 0.0f))
+                return;
+            const auto finite = [](float x) __attribute__((always_inline)) {
+                return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
+            };
+            uint32_t wild = 0;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!finite(o[r]))
+                {
+                    wild |= 1u << r;
+                    o[r] = __builtin_copysignf(__FLT_MAX__, o[r]);
+                }
+            const int lg = lane / 32;
+            const unsigned char *dims = vbase + 64 * dt;
+#pragma unroll 1
+            for (int64_t row0 = begin; row0 < end; row0 += kWave / 4) // four lanes a row
+            {
+                const int64_t row = row0 + lane / 4;
+                uint32_t top = 0;
+                if (row < end)
+                {
+                    const uint4 w = *reinterpret_cast<const uint4 *>(dims + row * vstride + 16 * (lane % 4));
+                    constexpr uint32_t kAbs = 0x7f807f80u, kOne = 0x00800080u;
+                    top = ((w.x & kAbs) + kOne) | ((w.y & kAbs) + kOne) | ((w.z & kAbs) + kOne) | ((w.w & kAbs) + kOne);
+                }
+                uint64_t rows = __ballot((top & 0x80008000u) != 0);
+                while (rows != 0)
+                {
+                    const int at = __builtin_ctzll(rows) / 4;
+                    rows &= ~(uint64_t{15} << (4 * at));
+                    const int64_t key = row0 + at;
+                    const bool seen = sees(static_cast<int32_t>(key));
+#pragma unroll
+                    for (int q4 = 0; q4 < 4; ++q4)
+                    {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(dims + key * vstride + 16 * q4 + 8 * lg);
+                        const float e[4] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
+#pragma unroll
+                        for (int u = 0; u < 4; ++u)
+                            o[4 * q4 + u] += seen && !finite(e[u]) ? e[u] : 0.0f;
+                    }
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((wild >> r & 1u) != 0 && finite(o[r]))
+                    o[r] = __builtin_copysignf(__builtin_huge_valf(), o[r]);
+        }
+
         // ---- results -------------------------------------------------------------------
 
         // Q fragments of the lane's column, a padding column's from the last position
@@ -824,7 +890,15 @@ namespace q3k
                     step(j + 1, k_b, v_b, s_b);
             }
             const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
-            const auto put_dims = [&](int dt, int first, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+            const auto sees = [&](int32_t key) __attribute__((always_inline)) {
+                if constexpr (TREE)
+                    return key < context || (tree >> ((key - context) & 31) & 1u) != 0;
+                else
+                    return key <= context + s_row;
+            };
+            const auto put_dims = [&](int dt, int first, f32x16_t part, float inv, float sum) __attribute__((always_inline)) {
+                if constexpr (!E4M3)
+                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, sees, part);
                 if (col_ok)
                     store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };
@@ -1187,7 +1261,15 @@ namespace q3k
             if constexpr (TREE)
                 query = query_of(tree.end[s_row]);
             const int64_t row = (b * a.S + s_col) * a.Hq + h_col;
-            const auto put_dims = [&](int dt, int first, const f32x16_t &part, float inv, float sum) __attribute__((always_inline)) {
+            const auto sees = [&](int32_t key) __attribute__((always_inline)) {
+                if constexpr (TREE)
+                    return key < context || (tree.mask[s_row][1 + (key - context) / 32] >> ((key - context) & 31) & 1u) != 0;
+                else
+                    return key <= context + s_row;
+            };
+            const auto put_dims = [&](int dt, int first, f32x16_t part, float inv, float sum) __attribute__((always_inline)) {
+                if constexpr (!E4M3)
+                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, sees, part);
                 if (col_ok)
                     store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };

@@ -101,3 +101,22 @@ def test_form_with_nan_rows(q3k, hip, form):
                 call.cache.poison(b, int(call.n[b]) - call.S - 1)
 
     _check(q3k, hip, "NaN rows", form, seed=1, edit=edit)
+
+
+@pytest.mark.parametrize("form", [c for c in cache_forms.FORMS if c[0] == "tree-bf16"] + [
+    ("tree-bf16", 3, 1, 8, 2, 200, True, "w4", "w4"), ("tree-bf16", 1, 1, 4, 1, 1, False, "w1", "w1"),
+    ("tree-bf16", 2, 40, 40, 1, 300, True, "generic", "generic")], ids=_id)
+def test_infinite_values(q3k, hip, form):
+    """Infinities of V in rows of the context, in the first and in later tiles, and of nodes: who sees the row gets the
+    infinity in that dim (NaN where two signs meet), and finite values in all others."""
+    def edit(call):
+        bits, values = call.cache.stored[1], call.cache.values[1]
+        for b in range(call.B):
+            n = int(call.n[b])
+            for i, row in enumerate(sorted({0, n // 3, n - call.S - 1, n - call.S, n - 1 - call.S // 2, n - 1} & set(range(n)))):
+                for dim, sign in (((29 * i + 3 * b) % D, 1), ((29 * i + 64 + b) % D, -1), (127, 1 if row % 2 else -1)):
+                    bits[b, row, :, dim] = 0x7F80 if sign > 0 else 0xFF80
+                    values[b, row, :, dim] = sign * np.inf
+        call.cache.upload()
+
+    _check(q3k, hip, "infinite V", form, seed=2, edit=edit)
