@@ -389,6 +389,8 @@ Q3K_API int q3k_kv_read_e4m3_bf16(const uint8_t *k_codes, const uint8_t *v_codes
  * device memory, may be NULL) of at least
  * q3k_cache_attention_workspace_bytes(...) bytes lets a launch split the key
  * range and merge the slices.  Calls that share a workspace must not overlap.
+ * Results are finite where V times the number of rows is below 2^119 in
+ * magnitude (and scores are finite); V past that may overflow the sum.
  */
 Q3K_API int q3k_gqa_attention_e4m3_bf16(const uint16_t *q, const uint8_t *k_codes,
                           const uint8_t *v_codes, const uint8_t *scales,
@@ -412,7 +414,7 @@ Q3K_API int q3k_gqa_attention_e4m3_bf16(const uint16_t *q, const uint8_t *k_code
  * sequence whose length is neither 0 (zeros) nor in [T, cached].  What rows
  * hold that a node does not attend to, NaN included, does not reach it; an
  * infinity of V in a row that it attends to (with a weight above 0) gives it
- * that infinity, NaN where both signs meet.
+ * that infinity, NaN where both signs meet.  Finite V are in range as above.
  * k_cache / v_cache are views as those of q3k_gqa_attention_bf16, [B, cached,
  * Hkv, D] by element strides; `cached` and the workspace are as in
  * q3k_gqa_attention_e4m3_bf16; the fast kernels take head_dim 128 with unit dim

@@ -120,3 +120,45 @@ def test_infinite_values(q3k, hip, form):
         call.cache.upload()
 
     _check(q3k, hip, "infinite V", form, seed=2, edit=edit)
+
+
+def _scale_v(call, power):
+    """V times 2^power: the scale bytes, or the exponents."""
+    c = call.cache
+    if c.e4m3:
+        c.bytes[..., 1] = np.where(c.bytes[..., 1] < 255, c.bytes[..., 1].astype(int) + power, 255)
+        v = ref.dequantise(c.stored[1], c.bytes[..., 1]).transpose(0, 2, 1, 3)
+    else:
+        bits = c.stored[1]
+        bits[:] = np.where((bits & 0x7FFF) > 0x7F80, bits, bits.astype(int) + power * 128)
+        v = ref.bf16(bits)
+    c.values[1] = np.where(np.isnan(v), 0.0, v)
+    c.upload()
+
+
+GENERIC = [(kind, 2, 3, 40, 1, 300, True, "generic", "generic") for kind in ("causal", "tree-bf16")]
+
+
+@pytest.mark.parametrize("form", [c for c in cache_forms.FORMS if c[5] <= 1500] + GENERIC, ids=_id)
+def test_largest_values(q3k, hip, form):
+    """V up to 2^119 over the number of rows, the least that overflows no sum of weights of up to 2^8, and of one sign in
+    half the dims."""
+    def edit(call):
+        c = call.cache
+        if c.e4m3:
+            c.stored[1][..., :64] &= 0x7F
+            _scale_v(call, int(np.floor(119 - np.log2(call.cached))) - 9 + 127 - 121)      # codes of up to 448 * 2^(121 - 127)
+        else:
+            c.stored[1][..., :64] &= 0x7FFF
+            _scale_v(call, int(np.floor(119 - np.log2(call.cached))) - 3)
+        most = np.abs(c.values[1]).max() * call.cached
+        assert 2.0**115 < most <= 2.0**119
+
+    _check(q3k, hip, "largest V", form, seed=3, edit=edit)
+
+
+@pytest.mark.parametrize("form", [c for c in cache_forms.FORMS if c[5] <= 1500] + GENERIC, ids=_id)
+def test_small_values(q3k, hip, form):
+    """V of rows whose largest value is about 2^-83: as exact as any other.  (Weights of 2^-16 of the largest and more have
+    their 16 bits there; what smaller ones lose, 2^-117 a row at most, is below 2^-20 of the result.)"""
+    _check(q3k, hip, "small V", form, seed=4, edit=lambda call: _scale_v(call, -84))
