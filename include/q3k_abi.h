@@ -383,9 +383,10 @@ Q3K_API int q3k_kv_read_e4m3_bf16(const uint8_t *k_codes, const uint8_t *v_codes
  * whose length lies outside [0, cached] gets NaN (the kernel reads nothing
  * there).  `cached` is what the host knows of the longest sequence, at most
  * seq_cap, and with lengths == NULL at least S: the launch is laid out for it,
- * so one captured in a graph serves every step up to it.  head_dim 128 with
- * 16-byte aligned q and codes and 2-byte aligned scales takes the matrix-core
- * kernels, anything up to 256 the generic one.  workspace (16-byte aligned
+ * so one captured in a graph serves every step up to it.  The matrix-core
+ * kernels take head_dim 128, at most 32 query heads a KV head, 16-byte aligned q
+ * and codes, 8-byte aligned out and 2-byte aligned scales; all else up to
+ * head_dim 256 goes to the generic kernel, many times slower.  workspace (16-byte aligned
  * device memory, may be NULL) of at least
  * q3k_cache_attention_workspace_bytes(...) bytes lets a launch split the key
  * range and merge the slices.  Calls that share a workspace must not overlap.
@@ -417,8 +418,8 @@ Q3K_API int q3k_gqa_attention_e4m3_bf16(const uint16_t *q, const uint8_t *k_code
  * that infinity, NaN where both signs meet.  Finite V are in range as above.
  * k_cache / v_cache are views as those of q3k_gqa_attention_bf16, [B, cached,
  * Hkv, D] by element strides; `cached` and the workspace are as in
- * q3k_gqa_attention_e4m3_bf16; the fast kernels take head_dim 128 with unit dim
- * stride and 16-byte aligned rows.
+ * q3k_gqa_attention_e4m3_bf16; the matrix-core kernels take what they take there,
+ * with unit dim stride and 16-byte aligned rows less than 2^25 bytes apart.
  */
 Q3K_API int q3k_gqa_tree_attention_bf16(const uint16_t *q, const uint16_t *k_cache,
                           const uint16_t *v_cache, uint16_t *out,

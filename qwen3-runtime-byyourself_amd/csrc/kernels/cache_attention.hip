@@ -1492,12 +1492,18 @@ namespace q3k
                                      : launch_block<2, 4, 1, E4M3, TREE>(what, a, B, stream);
         }
 
-        // Whether the matrix-core kernels take the call: rows and Q in 16-byte vectors, a
-        // tile's rows within 32-bit byte offsets.
+        // Whether the matrix-core kernels take calls of these sizes: a position's columns in
+        // one wave, tile ends counted in 32 bits.
+        bool fast_sizes(int32_t Hq, int32_t Hkv, int32_t D, int64_t cached)
+        {
+            return D == kAttD && Hq / Hkv <= kAttColsPerWave && cached <= INT32_MAX - 4 * kAttKeyTile;
+        }
+
+        // Whether they take the call: rows and Q in 16-byte vectors, a tile's rows within
+        // 32-bit byte offsets.
         bool fast(const CacheArgs &a, bool e4m3)
         {
-            // (tile ends are counted in 32 bits)
-            if (a.D != kAttD || a.Hq / a.Hkv > kAttColsPerWave || a.cached > INT32_MAX - 4 * kAttKeyTile)
+            if (!fast_sizes(a.Hq, a.Hkv, a.D, a.cached))
                 return false;
             if (!aligned16(a.q) || !aligned16(a.k) || !aligned16(a.v) || !aligned_to(a.out, 8))
                 return false;
@@ -1714,7 +1720,7 @@ extern "C" int q3k_gqa_tree_attention_e4m3_bf16(const uint16_t *q, const uint8_t
 
 extern "C" int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S, int32_t Hq, int32_t Hkv, int32_t D, int64_t cached)
 {
-    if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D != q3k::kAttD || cached <= 0 || cached > INT32_MAX ||
+    if (B <= 0 || S <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || cached <= 0 || !q3k::fast_sizes(Hq, Hkv, D, cached) ||
         S > INT64_MAX / B || B * S > INT64_MAX / Hq || B * S * Hq > INT32_MAX)
         return 0;
     return q3k::cache_attention_workspace_bytes(B, S, Hq, Hkv, cached);

@@ -67,3 +67,13 @@ def test_plain_form_agrees_with_the_other():
         assert np.array_equal(np.isnan(got), np.isnan(want)) and np.array_equal(got[np.isinf(want)], want[np.isinf(want)])
         some = np.isfinite(want) & np.isfinite(most)
         assert some.sum() > 100 and np.abs(got - want)[some].max() < 1e-13 and np.abs(bound - most)[some].max() < 1e-13
+
+
+def test_workspace_query_of_calls_that_never_split(q3k):
+    """The generic kernel takes more than 32 query heads a KV head, other widths and lengths whose tiles' ends pass 2^31;
+    it cuts no keys, so its calls need no workspace."""
+    ws = q3k.cache_attention_workspace_bytes
+    assert ws(1, 1, 32, 1, 128, 8192) > 0
+    for args in ((1, 1, 33, 1, 128, 8192), (1, 1, 40, 1, 128, 8192), (2, 30, 128, 2, 128, 5000), (1, 1, 32, 1, 96, 8192),
+                 (1, 1, 32, 1, 128, 2**31 - 1)):
+        assert ws(*args) == 0
