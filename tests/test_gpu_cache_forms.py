@@ -37,13 +37,15 @@ class _CodesCache(_Cache):
 class _Call:
     """One of cache_forms.FORMS with its inputs; rows of the cache past a sequence's length hold NaN."""
 
-    def __init__(self, hip, form, seed=0, edit=None):
+    def __init__(self, hip, form, seed=0, edit=None, lengths=None):
         self.hip = hip
         kind, self.B, self.S, self.Hq, self.Hkv, self.cached, ragged = form[:7]
         B, S = self.B, self.S
         rng = np.random.default_rng(seed + B + 31 * S + self.cached)
-        self.lengths = cache_forms.lengths_of(B, S, self.cached, ragged)
-        self.n = np.full(B, self.cached) if self.lengths is None else self.lengths
+        self.lengths = lengths if lengths is not None else cache_forms.lengths_of(B, S, self.cached, ragged)
+        given = np.full(B, self.cached) if self.lengths is None else np.asarray(self.lengths)
+        self.bad = (given < 0) | (given > self.cached) | ((given > 0) & (given < S) & (kind != "causal"))
+        self.n = np.where(self.bad, 0, given)
         if kind == "tree-bf16":
             self.cache = _Cache(hip, rng, False, B, self.Hkv, D, self.cached + 3, self.n)
         else:
@@ -53,7 +55,7 @@ class _Call:
         if edit is not None:
             edit(self)
         self.bq, = _up(hip, self.q)
-        self.bl = _up(hip, np.asarray(self.lengths, np.int32))[0] if ragged else None
+        self.bl = _up(hip, np.asarray(self.lengths, np.int32))[0] if self.lengths is not None else None
         self.bp = (_up(hip, self.trees)[0], S) if self.trees is not None else None
 
     def shape(self):
@@ -68,9 +70,13 @@ class _Call:
     def want(self):
         x = ref.bf16(self.q).reshape(self.q.shape)
         k, v = self.cache.values
-        pairs = [cache_forms.attention(x[b], k[b, :n], v[b, :n], int(n), self.S, None if self.trees is None else self.trees[b])
-                 for b, n in enumerate(self.n)]
-        return np.stack([p[0] for p in pairs]), np.stack([p[1] for p in pairs])
+        out, bound = np.zeros(x.shape), np.zeros(x.shape)
+        out[self.bad] = np.nan
+        for b, n in enumerate(self.n):
+            if n > 0:
+                tree = None if self.trees is None else self.trees[b]
+                out[b], bound[b] = cache_forms.attention(x[b], k[b, :n], v[b, :n], int(n), self.S, tree)
+        return out, bound
 
 
 def _check(q3k, hip, name, form, **kw):
@@ -120,6 +126,29 @@ def test_infinite_values(q3k, hip, form):
         call.cache.upload()
 
     _check(q3k, hip, "infinite V", form, seed=2, edit=edit)
+
+
+@pytest.mark.parametrize("form", [c for c in cache_forms.FORMS if c[6] and c[1] >= 12], ids=_id)
+def test_form_with_odd_lengths(q3k, hip, form):
+    """No rows, one, fewer than the queries (before whose first row some see nothing), below 0, past the cache's."""
+    kind, B, S, cached = form[0], form[1], form[2], form[5]
+    lengths = cache_forms.lengths_of(B, S, cached, True)
+    lengths[:8] = [0, 1, -1, cached + 1, S // 2, S, cached - 1, -2**31]
+    _check(q3k, hip, f"odd lengths {kind}", form, seed=5, lengths=lengths)
+
+
+@pytest.mark.parametrize("kind", ["causal", "tree", "tree-bf16"])
+@pytest.mark.parametrize("S", [1, 5, 40])
+def test_one_long_sequence_among_short_ones(q3k, hip, kind, S):
+    lengths = np.full(40, S + 19, np.int32)
+    lengths[::3] = S + 50
+    lengths[23] = 9001
+    _check(q3k, hip, "one long", (kind, 40, S, 8, 2, 9001, True, "", ""), seed=6, lengths=lengths)
+
+
+def test_whole_prompt(q3k, hip):
+    """Thousands of queries: every causal query block of a long prompt, the first of which sees one tile."""
+    _check(q3k, hip, "prompt", ("causal", 1, 4099, 8, 2, 4099, False, "", ""), seed=7)
 
 
 def _scale_v(call, power):
