@@ -337,8 +337,9 @@ Q3K_API int q3k_qk_norm_rope_kv_append_bf16(uint16_t *q, const uint16_t *k,
  * A row (one position, one KV head) holds x[d] = code[d] * scale.  It is
  * written with the smallest scale 2^e, e >= -126, for which no finite |x[d]|
  * exceeds 448 * 2^e, and code = RNE(x * 2^-e); the scaling is exact, so the
- * code's rounding (half a step, 2^-4 of the value) is the only one, and every
- * value read back is a bf16 value.  An infinity or a NaN becomes a NaN code
+ * code's rounding is the only one (half a step: 2^-4 of the value down to 2^-6
+ * of the scale, 2^-10 of the scale below that, where codes are subnormal), and
+ * every value read back is a bf16 value.  An infinity or a NaN becomes a NaN code
  * (e4m3 has no infinity) and does not count for the scale.  Scale bytes 0 and
  * 255 are never written.  A head's rows lie together (in the bf16 cache a
  * position's heads do): attention reads one head's rows, 5.4-5.9 TB/s so and
@@ -444,7 +445,8 @@ Q3K_API int q3k_gqa_tree_attention_e4m3_bf16(const uint16_t *q,
  * Workspace bytes that let the three attention calls above split the key range
  * of up to `cached` rows (S queries or tree nodes a sequence; 0: they split
  * none): one of the size for the cache's length serves every shorter one of the
- * same B, S and heads.
+ * same B, S and heads.  It is a bound for all three and every length; a call may
+ * take less, or none.
  */
 Q3K_API int64_t q3k_cache_attention_workspace_bytes(int64_t B, int64_t S,
                           int32_t Hq, int32_t Hkv, int32_t D, int64_t cached);

@@ -21,6 +21,10 @@
 //   into the weights instead (there a lane holds one column and 16 keys of each 32).
 //   More columns (larger trees, prefill): a block of waves shares its K and V tiles
 //   as bf16; codes are converted once, on their way into LDS.
+// A weight meets V as a bf16 part and a bf16 remainder, 2^-18 of it at most away from
+// fp32: beside fp32 weights single results move by one bf16 step (6e-5 to 1.1e-4 of the
+// norm of a result) and the error against 64 bits stays the output's rounding.  A third
+// part would be half as many products again.
 // The mask only touches the tiles at a sequence's end.  A masked score is -inf, so
 // what K holds in a row that a query does not see never counts.  What V holds there
 // meets a weight of zero, and zero times an infinity or a NaN is NaN: so a masked
@@ -36,8 +40,9 @@
 // Generic path (any head_dim <= 256, any strides and alignment): one wave per
 // query row, its rows in order, lanes over the head dimension, the running
 // maximum and sum of the softmax in fp32.  It is bound by the chain of one row after
-// another and reads K and V once for each query head: 50 to 500 times the time of the
-// others where both could run (64 ragged sequences of up to 4096 rows: 4674 us, 66).
+// another and reads K and V once for each query head: 60 to 700 times the time of the
+// others where both could run (64 ragged sequences of up to 4096 rows: 4674 us, 69; one
+// of 8191: 7714 us, 10.7).
 #include "attention_tiles.hpp"
 #include "dispatch.hpp"
 #include "kv_e4m3.hpp"
@@ -106,9 +111,11 @@ namespace q3k
         // heads: 66.4 us, 78.0 in a random order; of 4000 to 16000 rows 231 us and 278; their
         // trees of 5 nodes over up to 2053 bf16 rows 64.7 us and 73.8).  Finding the
         // place takes 0.6 to 1 us, more than it gives sequences that are cut into slices (4 of
-        // up to 8000 rows: 17.3 us, 18.4 ordered).  In the block kernels, two blocks to a CU, it gave nothing
-        // (16 trees of 64 nodes, 40 heads: 124 to 130 us, 122 in a random order).  Of more
-        // than 64 sequences each 64 are ordered among themselves.
+        // up to 8000 rows: 17.3 us, 18.4 ordered).  In the block kernels it gave nothing where
+        // the longest sequence's chain of tiles sets the time (16 trees of 64 nodes, 40 heads,
+        // one key group, two blocks to a CU: 124 to 130 us, 122 in a random order); with two
+        // key groups it was not tried.  Of more than 64 sequences each 64 are ordered among
+        // themselves.
         __device__ __forceinline__ int32_t sequence_at(const CacheArgs &a, int32_t rank, int lane)
         {
             if (!a.ordered)
@@ -943,7 +950,8 @@ namespace q3k
         //   or cost the second block of a CU).
         // What bounds it is the softmax beside the matrix instructions, as in the bf16
         // attention.  512 queries over 8192 rows, 32 / 8 heads, e4m3, in 4 slices: 95 to 101 us
-        // and 8 for the merge, 590 to 640 TFLOP/s of the products, matrix cores busy 44%.  16
+        // and 8 for the merge, together 610 to 640 TFLOP/s of the products, matrix cores busy
+        // 44%.  16
         // ragged trees of 64 nodes over up to 4160 bf16 rows, 40 / 8 heads: 116 to 122 us, 440
         // to 465 TFLOP/s, 384 blocks of unequal length, two to a CU.  Four groups with 64 columns
         // are for few blocks (4 trees of 64 nodes over 2000 rows: 38.4 us, 40.7 with 128

@@ -3,8 +3,9 @@
 //
 // A wave owns a few chunks of one (layer, sequence): a chunk is up to 64 words of a
 // head's K or V rows, and where a row is narrower (128 bytes of codes: 8 words) the
-// lanes hold that many entries of the path side by side.  It moves them kStep
-// entries at a time, all loads before the stores.  An entry is only followed where
+// lanes hold that many entries of the path side by side.  It moves eight entries of one
+// chunk at a time, or where rows are narrow one step of entries of eight chunks, all
+// loads before the stores.  An entry is only followed where
 // path[b, i] >= i, so whatever is read from row i belongs to an entry at or before
 // i: its load was issued with or before that of entry i, and the store to row i
 // waits for that one.  So rows may overlap and no second buffer is needed.
