@@ -543,18 +543,19 @@ namespace q3k
         // and a remainder of zero, or below it, times an infinity is NaN, not the infinity.
         // So where dims 32 dt .. + 31 of a result (elements of o as store_dims takes them)
         // are not finite, the wave looks through rows begin .. end - 1 of V again and gives
-        // each such element the sum of the infinities and NaN that its column sees.  What
-        // they do not explain has left fp32's range, and stays infinite.  Only bf16 holds
-        // infinities.  Looking costs 16 instructions where all is finite, once a result.
+        // each such element the sum of the infinities and NaN that its column sees, until all
+        // are NaN.  What they do not explain has left fp32's range, and stays infinite.  live:
+        // whether the lane's column has a result that l does not make NaN anyway.  Only bf16
+        // holds infinities.  Looking costs 16 instructions where all is finite, once a result.
         template <typename Sees>
         __device__ __forceinline__ void see_infinities(const unsigned char *vbase, int32_t vstride, int32_t begin, int32_t end,
-                                                       int dt, int lane, Sees sees, f32x16_t &o)
+                                                       int dt, int lane, bool live, Sees sees, f32x16_t &o)
         {
             float zero = 0.0f; // NaN if one is not finite
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 zero = __builtin_fmaf(o[r], 0.0f, zero);
-            if (!__any(zero != 0.0f))
+            if (!__any(live && zero != 0.0f))
                 return;
             const auto finite = [](float x) __attribute__((always_inline)) {
                 return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u;
@@ -562,7 +563,7 @@ namespace q3k
             uint32_t wild = 0;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if (!finite(o[r]))
+                if (live && !finite(o[r]))
                 {
                     wild |= 1u << r;
                     o[r] = __builtin_copysignf(__FLT_MAX__, o[r]);
@@ -581,6 +582,7 @@ namespace q3k
                     top = ((w.x & kAbs) + kOne) | ((w.y & kAbs) + kOne) | ((w.z & kAbs) + kOne) | ((w.w & kAbs) + kOne);
                 }
                 uint64_t rows = __ballot((top & 0x80008000u) != 0);
+                bool open = rows == 0; // whether another row could change an element
                 while (rows != 0)
                 {
                     const int at = __builtin_ctzll(rows) / 4;
@@ -597,6 +599,11 @@ namespace q3k
                             o[4 * q4 + u] += seen && !finite(e[u]) ? e[u] : 0.0f;
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    open = open || ((wild >> r & 1u) != 0 && o[r] == o[r]);
+                if (!__any(open))
+                    break;
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -910,7 +917,7 @@ namespace q3k
             };
             const auto put_dims = [&](int dt, int first, f32x16_t part, float inv, float sum) __attribute__((always_inline)) {
                 if constexpr (!E4M3)
-                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, sees, part);
+                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, col_ok && query == Query::Sees && sum == sum, sees, part);
                 if (col_ok)
                     store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };
@@ -1282,7 +1289,7 @@ namespace q3k
             };
             const auto put_dims = [&](int dt, int first, f32x16_t part, float inv, float sum) __attribute__((always_inline)) {
                 if constexpr (!E4M3)
-                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, sees, part);
+                    see_infinities(vbase, vstride, k_begin, k_end, dt, lane, col_ok && query == Query::Sees && sum == sum, sees, part);
                 if (col_ok)
                     store_dims<KW == 8 ? 2 : 4>(a, split, sp, row, dt, first, lg, part, inv, sum, query);
             };

@@ -191,3 +191,19 @@ def test_small_values(q3k, hip, form):
     """V of rows whose largest value is about 2^-83: as exact as any other.  (Weights of 2^-16 of the largest and more have
     their 16 bits there; what smaller ones lose, 2^-117 a row at most, is below 2^-20 of the result.)"""
     _check(q3k, hip, "small V", form, seed=4, edit=lambda call: _scale_v(call, -84))
+
+
+@pytest.mark.parametrize("what", ["V", "Q"])
+@pytest.mark.parametrize("S", [1, 5, 40])
+def test_nan_everywhere(q3k, hip, S, what):
+    """V, or the queries, NaN as a whole, and empty nodes that stay zeros."""
+    def edit(call):
+        if what == "Q":
+            call.q[:] = 0x7FC0
+            return
+        for b in range(call.B):
+            call.cache.stored[1][b, :call.n[b]] = 0x7FC0
+        call.cache.values[1][:] = np.nan
+        call.cache.upload()
+
+    _check(q3k, hip, f"NaN {what}", ("tree-bf16", 2, S, 8, 2, 1500, False, "", ""), seed=8, edit=edit)
